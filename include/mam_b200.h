@@ -362,6 +362,57 @@ size_t mam_colsum_workspace_bytes(int64_t M, int64_t N);
 int mam_colsum_f32(const float* in, float* out, int64_t M, int64_t N, void* workspace, size_t workspace_bytes,
                    void* stream);
 
+/* ---- Operators between the MAM layers of a transformer block ----
+ * Layer norm, dropout with a residual addition, and GELU, on fp32, fp16 or bf16 tensors (the arithmetic is fp32, each
+ * output rounded once).  They stand where the reference's ViT example uses torch.nn.LayerNorm, GELU and Dropout
+ * (examples/vitb16_imagenet1k/utils.py:67-77 swaps the dense layers between them).
+ *
+ * Dropout: element i (counted in the tensor's contiguous order) is dropped where its 32-bit draw is below
+ * drop_rate * 2^32, else multiplied by 1 / (1 - drop_rate); 0 <= drop_rate < 1.  The draw is a function of (seed, i), so no
+ * mask is stored and the backward forms it again; seed = drop_seed, plus *drop_seed_at where that pointer (device memory,
+ * 8-byte aligned) is given, which the kernels read: a captured graph takes a new mask at each replay when the value there
+ * is advanced between them.  The draws are not those of mam_drop_f32.
+ *
+ * Pointers are aligned to their type; 16-byte alignment and widths that are multiples of 16 bytes make the calls faster.
+ * Outputs must not overlap inputs. */
+#define MAM_F32 0
+#define MAM_F16 1
+#define MAM_BF16 2
+
+/* Layer norm over the last dimension of [rows, width]:
+ *   residual == NULL:  s = x, sum must be NULL and drop_rate 0
+ *   else               s = residual + drop(x), stored in sum [rows, width], rounded to the type
+ *   y = (s - mean(s)) / sqrt(mean((s - mean(s))^2) + eps) * weight + bias     (weight NULL: ones, bias NULL: zeros)
+ * Rows of x and residual are x_pitch and residual_pitch elements apart; y and sum are contiguous.  param_dtype (of weight
+ * and bias) is MAM_F32 or dtype.  stats, if not NULL, takes 2 * rows floats for the backward (8-byte aligned).
+ * Limits: rows < 2^31, width <= 2^30. */
+int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int64_t residual_pitch,
+                       const void* weight, const void* bias, int param_dtype, float eps,
+                       float drop_rate, uint64_t drop_seed, const int64_t* drop_seed_at,
+                       void* y, void* sum, float* stats, int64_t rows, int64_t width, int dtype, void* stream);
+
+/* Its backward, from s (x or sum, rows s_pitch apart) and stats.  gy: gradient of y; gsum: gradient of sum; either may be
+ * NULL (zeros).  ds: gradient of s, which is the residual's too.  dx, required where drop_rate > 0: drop(ds), the gradient
+ * of x; else NULL, and ds is the gradient of x.  dweight and dbias, each optional, in param_dtype: summed in a fixed order;
+ * with either of them the call needs the workspace (256-byte aligned). */
+size_t mam_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
+int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t s_pitch, const float* stats,
+                       const void* weight, int param_dtype,
+                       float drop_rate, uint64_t drop_seed, const int64_t* drop_seed_at,
+                       void* ds, void* dx, void* dweight, void* dbias, int64_t rows, int64_t width, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = residual + drop(x), residual optional.  With the gradient in the place of x and no residual it is its own
+ * backward. */
+int mam_dropout_add(const void* x, const void* residual, void* y, int64_t n, int dtype,
+                    float drop_rate, uint64_t drop_seed, const int64_t* drop_seed_at, void* stream);
+
+/* y = drop(x * Phi(x)), Phi the normal distribution's integral (the exact GELU); dx = drop(gy * (Phi(x) + x Phi'(x))). */
+int mam_gelu_fwd(const void* x, void* y, int64_t n, int dtype,
+                 float drop_rate, uint64_t drop_seed, const int64_t* drop_seed_at, void* stream);
+int mam_gelu_bwd(const void* gy, const void* x, void* dx, int64_t n, int dtype,
+                 float drop_rate, uint64_t drop_seed, const int64_t* drop_seed_at, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -49,7 +49,7 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
     srcs = _sources((".cu", ".cuh"))
     if force or _stale(LIB, srcs):
         cus = [s for s in srcs if s.endswith(".cu")]
-        cmd = [_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB, *cus]
+        cmd = [_nvcc(), *NVCC_FLAGS, "--threads", "0", "-shared", "-o", LIB, *cus]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         subprocess.check_call(cmd, cwd=CSRC)
@@ -57,8 +57,8 @@ def build_lib(force: bool = False, verbose: bool = False) -> str:
 
 
 def build_shim(force: bool = False) -> str:
-    src = os.path.join(CSRC, "torch_shim.cpp")
-    if force or _stale(SHIM, [src, os.path.join(HERE, "..", "include", "mam_b200.h"), LIB]):
+    srcs = [os.path.join(CSRC, "torch_shim.cpp"), os.path.join(CSRC, "torch_block.cpp")]
+    if force or _stale(SHIM, [*srcs, os.path.join(HERE, "..", "include", "mam_b200.h"), LIB]):
         import torch
         from torch.utils import cpp_extension as ce
 
@@ -67,7 +67,7 @@ def build_shim(force: bool = False) -> str:
             inc += ["-I", p]
         tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
         cxx = "g++"
-        cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-o", SHIM, src, *inc,
+        cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-o", SHIM, *srcs, *inc,
                "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
                "-L", tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
                "-L", HERE, "-l:libmam_b200.so",

@@ -60,6 +60,12 @@ ABI = {
     "mam_spmm_csr_ws_f32": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
     "mam_colsum_workspace_bytes": (_sz, [_i64, _i64]),
     "mam_colsum_f32": (_i32, [_vp, _vp, _i64, _i64, _vp, _sz, _vp]),
+    "mam_layer_norm_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _f32, _f32, ctypes.c_uint64, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "mam_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "mam_layer_norm_bwd": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _i32, _f32, ctypes.c_uint64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp, _sz, _vp]),
+    "mam_dropout_add": (_i32, [_vp, _vp, _vp, _i64, _i32, _f32, ctypes.c_uint64, _vp, _vp]),
+    "mam_gelu_fwd": (_i32, [_vp, _vp, _i64, _i32, _f32, ctypes.c_uint64, _vp, _vp]),
+    "mam_gelu_bwd": (_i32, [_vp, _vp, _vp, _i64, _i32, _f32, ctypes.c_uint64, _vp, _vp]),
     "mam_transpose_f32": (_i32, [_vp, _vp, _i64, _i64, _vp]),
 }
 

@@ -17,44 +17,13 @@
 #include "mam_fwd_generic.cuh"
 #include "mam_fwd_sliced.cuh"
 #include "mam_fwd_tiled.cuh"
+#include "mam_host.cuh"
 
 using namespace mamb200;
 
 namespace {
 
-thread_local cudaError_t t_last_cuda = cudaSuccess;
 __device__ int g_wait_gave_up = 0;  // set by kernels whose bounded wait ran out
-
-int cuda_fail(cudaError_t e) {
-    t_last_cuda = e;
-    return MAM_ERR_CUDA;
-}
-#define MAM_CUDA(x)                                  \
-    do {                                             \
-        cudaError_t e_ = (x);                        \
-        if (e_ != cudaSuccess) return cuda_fail(e_); \
-    } while (0)
-
-struct DevInfo {
-    int valid = 0, sms = 0, major = 0, minor = 0, max_smem = 0;
-};
-DevInfo g_dev[64];
-
-int device_info(const DevInfo** out) {
-    int dev = 0;
-    MAM_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
-    DevInfo& d = g_dev[dev];
-    if (!d.valid) {
-        MAM_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
-        MAM_CUDA(cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, dev));
-        MAM_CUDA(cudaDeviceGetAttribute(&d.minor, cudaDevAttrComputeCapabilityMinor, dev));
-        MAM_CUDA(cudaDeviceGetAttribute(&d.max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev));
-        d.valid = 1;
-    }
-    *out = &d;
-    return d.major == 10 ? MAM_OK : MAM_ERR_NOT_SM100;
-}
 
 // What the size queries plan with: the current device, or a B200's 148 SMs where there is none (they need no GPU).
 DevInfo plan_dev() {
@@ -245,8 +214,6 @@ static __device__ __align__(256) unsigned char g_static_scratch[MAM_STATIC_SCRAT
 void* g_static_scratch_addr[64] = {nullptr};  // device address per device, looked up on first use
 std::mutex g_static_scratch_mutex;
 
-int bad_ptr(const void* p) { return p == nullptr; }
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 size_t round256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // K not a multiple of 4: both operands are copied once with padded rows (mam_stage_ragged_kernel) so that TMA can
@@ -749,16 +716,6 @@ int mam_nchw_to_nhwc_f32(const float* x, float* out, int64_t B, int64_t C, int64
     MAM_CUDA(cudaGetLastError());
     return MAM_OK;
 }
-
-namespace {
-// rate in [0, 1) -> threshold on a 32-bit draw; false if the rate is out of range
-bool drop_threshold(float rate, unsigned* thr) {
-    if (!(rate >= 0.f && rate < 1.f)) return false;
-    const double t = (double)rate * 4294967296.0;
-    *thr = t >= 4294967295.0 ? 4294967295u : (unsigned)t;
-    return true;
-}
-}  // namespace
 
 int mam_fwd_f32(const float* a, const float* b, int b_layout, const float* bias, const float* dense, int blend,
                 float alpha, float beta, float* y, int32_t* argmax, int32_t* argmin, int64_t M, int64_t K,

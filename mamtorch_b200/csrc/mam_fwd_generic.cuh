@@ -9,6 +9,7 @@
 // with -inf/+inf, and handles ragged edges by clamping the load coordinates: a replicated element
 // can tie but never beat the original, so it never changes a value or an index.
 #pragma once
+#include "mam_drop.cuh"
 #include "mam_ptx.cuh"
 
 namespace mamb200 {
@@ -24,18 +25,6 @@ struct EpilogueArgs {
     unsigned drop_threshold;   // rate * 2^32
     float drop_scale;          // 1 / (1 - rate); 0 = no dropout
 };
-
-// The keep / drop decision of element `idx` under `seed`: a counter-based generator (the splitmix64 mixing
-// function on seed + idx * golden ratio), so that the same mask is formed again wherever it is needed --
-// forward epilogue, backward, weight drop -- without ever being stored.  Dropped with probability
-// threshold / 2^32.
-__device__ __forceinline__ bool mam_drop_keeps(unsigned long long seed, unsigned long long idx, unsigned threshold) {
-    unsigned long long z = seed + idx * 0x9E3779B97F4A7C15ull;
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    z ^= z >> 31;
-    return (unsigned)(z >> 32) >= threshold;
-}
 
 // out[i] = in[i] * scale where element i is kept, else 0 (in == out is fine)
 __global__ void __launch_bounds__(256)

@@ -1,0 +1,53 @@
+// Host-side helpers shared by the translation units of libmam_b200.so: error recording and device attributes.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "../../include/mam_b200.h"
+
+namespace mamb200 {
+
+inline thread_local cudaError_t t_last_cuda = cudaSuccess;
+
+inline int cuda_fail(cudaError_t e) {
+    t_last_cuda = e;
+    return MAM_ERR_CUDA;
+}
+#define MAM_CUDA(x)                                  \
+    do {                                             \
+        cudaError_t e_ = (x);                        \
+        if (e_ != cudaSuccess) return cuda_fail(e_); \
+    } while (0)
+
+struct DevInfo {
+    int valid = 0, sms = 0, major = 0, minor = 0, max_smem = 0;
+};
+inline DevInfo g_dev[64];
+
+inline int device_info(const DevInfo** out) {
+    int dev = 0;
+    MAM_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
+    DevInfo& d = g_dev[dev];
+    if (!d.valid) {
+        MAM_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
+        MAM_CUDA(cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, dev));
+        MAM_CUDA(cudaDeviceGetAttribute(&d.minor, cudaDevAttrComputeCapabilityMinor, dev));
+        MAM_CUDA(cudaDeviceGetAttribute(&d.max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev));
+        d.valid = 1;
+    }
+    *out = &d;
+    return d.major == 10 ? MAM_OK : MAM_ERR_NOT_SM100;
+}
+
+inline int bad_ptr(const void* p) { return p == nullptr; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// rate in [0, 1) -> threshold on a 32-bit draw; false if the rate is out of range
+inline bool drop_threshold(float rate, unsigned* thr) {
+    if (!(rate >= 0.f && rate < 1.f)) return false;
+    const double t = (double)rate * 4294967296.0;
+    *thr = t >= 4294967295.0 ? 4294967295u : (unsigned)t;
+    return true;
+}
+
+}  // namespace mamb200

@@ -1,0 +1,373 @@
+// PyTorch operators over the layer norm, dropout and GELU entry points of the C ABI, in the `mamtorch_b200` namespace.
+//
+// The `*_forward` / `*_backward` operators validate, allocate and call the library (CUDA only: a CPU tensor gets the
+// dispatcher's NotImplementedError).  The differentiable ones (layer_norm, dropout_add_layer_norm, dropout, gelu) call
+// them below a C++ autograd node where a gradient is wanted, and directly where none is: for a few rows the host's time
+// is the call's time.
+#include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include <vector>
+
+#include "../../include/mam_b200.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void check_status(int st, const char* what) {
+    if (st == MAM_OK) return;
+    TORCH_CHECK(false, what, ": ", mam_status_str(st), st == MAM_ERR_CUDA ? ": " : "",
+                st == MAM_ERR_CUDA ? mam_last_cuda_error() : "");
+}
+
+bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* mut(Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+
+int dtype_code(const Tensor& t, const char* name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return MAM_F32;
+        case at::kHalf: return MAM_F16;
+        case at::kBFloat16: return MAM_BF16;
+        default: TORCH_CHECK(false, name, " must be float32, float16 or bfloat16, not ", t.scalar_type());
+    }
+}
+void check_like(const Tensor& t, const Tensor& x, const char* name) {
+    TORCH_CHECK(t.device() == x.device(), name, " must be on the device of x");
+    TORCH_CHECK(t.scalar_type() == x.scalar_type(), name, " must have the dtype of x");
+    TORCH_CHECK(t.sizes() == x.sizes(), name, " must have the shape of x");
+}
+// weight and bias: one value a column, fp32 or the dtype of x, both of the same; their dtype code
+int check_params(const Tensor& x, const Tensor& weight, const Tensor& bias) {
+    int code = -1;
+    const int own = dtype_code(x, "x");
+    for (const Tensor* t : {&weight, &bias}) {
+        if (!t->defined()) continue;
+        TORCH_CHECK(t->device() == x.device(), "weight and bias must be on the device of x");
+        TORCH_CHECK(t->dim() == 1 && t->size(0) == x.size(-1), "weight and bias must have one value per column of x");
+        const int c = dtype_code(*t, "weight and bias");
+        TORCH_CHECK(c == own || c == MAM_F32, "weight and bias must be float32 or have the dtype of x");
+        TORCH_CHECK(code < 0 || code == c, "weight and bias must have the same dtype");
+        code = c;
+    }
+    return code < 0 ? own : code;
+}
+void check_drop(const Tensor& x, double rate, const OptTensor& seed_at) {
+    TORCH_CHECK(rate >= 0.0 && rate < 1.0, "drop_rate must be in [0, 1)");
+    if (has(seed_at))
+        TORCH_CHECK(seed_at->device() == x.device() && seed_at->scalar_type() == at::kLong && seed_at->numel() == 1,
+                    "a drop_seed tensor must hold one int64 on the device of x");
+}
+const int64_t* seed_ptr(const OptTensor& seed_at) { return has(seed_at) ? seed_at->const_data_ptr<int64_t>() : nullptr; }
+
+// t[..., width] as rows with a uniform distance: in place where its strides are such, else a contiguous copy
+Tensor as_rows(const Tensor& t, int64_t& pitch) {
+    const int64_t width = t.size(-1);
+    pitch = width;
+    if (t.is_contiguous()) return t;
+    if (t.stride(-1) == 1 || width == 1) {
+        int64_t step = -1, expect = -1;   // of the innermost leading dimension that is longer than one; of the next
+        bool uniform = true;
+        for (int64_t i = t.dim() - 2; i >= 0; --i) {
+            if (t.size(i) == 1) continue;
+            if (step < 0) step = t.stride(i);
+            else if (t.stride(i) != expect) uniform = false;
+            expect = t.stride(i) * t.size(i);
+        }
+        if (uniform && (step < 0 || step >= width)) {
+            if (step >= 0) pitch = step;
+            return t;
+        }
+    }
+    return t.contiguous();
+}
+
+// ---------------------------------------------------------------- CUDA operators
+
+std::vector<Tensor> layer_norm_forward(const Tensor& x, const OptTensor& residual, const OptTensor& weight,
+                                       const OptTensor& bias, double eps, double rate, int64_t seed,
+                                       const OptTensor& seed_at, bool want_stats) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dtype = dtype_code(x, "x");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have a last dimension to normalise");
+    TORCH_CHECK(eps >= 0.0, "eps must not be negative");
+    const Tensor w = has(weight) ? weight->contiguous() : Tensor(), b = has(bias) ? bias->contiguous() : Tensor();
+    const int pdtype = check_params(x, w, b);
+    check_drop(x, rate, seed_at);
+    if (has(residual)) check_like(*residual, x, "residual");
+    else TORCH_CHECK(rate == 0.0, "dropout before the norm needs a residual");
+    c10::cuda::CUDAGuard guard(x.device());
+    int64_t xp = 0, rp = 0;
+    const Tensor xr = as_rows(x, xp), rr = has(residual) ? as_rows(*residual, rp) : Tensor();
+    const int64_t width = x.size(-1), rows = x.numel() / width;
+    std::vector<Tensor> out{at::empty(x.sizes(), x.options())};
+    if (rr.defined()) out.push_back(at::empty(x.sizes(), x.options()));
+    if (want_stats) out.push_back(at::empty({rows, 2}, x.options().dtype(at::kFloat)));
+    if (rows == 0) return out;
+    check_status(mam_layer_norm_fwd(ptr(xr), xp, ptr(rr), rp, ptr(w), ptr(b), pdtype, (float)eps, (float)rate,
+                                    (uint64_t)seed, seed_ptr(seed_at), mut(out[0]), rr.defined() ? mut(out[1]) : nullptr,
+                                    want_stats ? out.back().mutable_data_ptr<float>() : nullptr, rows, width, dtype,
+                                    at::cuda::getCurrentCUDAStream().stream()),
+                 "mam_layer_norm_fwd");
+    return out;
+}
+
+// ds, dx (where something is dropped; else ds is the gradient of x too), dweight, dbias; those not wanted are empty
+std::vector<Tensor> layer_norm_backward(const OptTensor& gy, const OptTensor& gsum, const Tensor& s, const Tensor& stats,
+                                        const OptTensor& weight, double rate, int64_t seed, const OptTensor& seed_at,
+                                        bool params_f32, bool want_weight, bool want_bias) {
+    TORCH_CHECK(s.is_cuda(), "s must be a CUDA tensor");
+    const int dtype = dtype_code(s, "s");
+    TORCH_CHECK(s.dim() >= 1 && s.size(-1) > 0, "s must have a last dimension to normalise");
+    const int64_t width = s.size(-1), rows = s.numel() / width;
+    TORCH_CHECK(stats.device() == s.device() && stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
+                    stats.numel() == 2 * rows,
+                "stats must be the forward's");
+    const Tensor w = has(weight) ? weight->contiguous() : Tensor();
+    const int pdtype = w.defined() ? check_params(s, w, Tensor()) : params_f32 ? MAM_F32 : dtype;
+    TORCH_CHECK((pdtype == MAM_F32) == (params_f32 || dtype == MAM_F32), "params_f32 and the dtype of weight differ");
+    check_drop(s, rate, seed_at);
+    if (has(gy)) check_like(*gy, s, "the gradient of y");
+    if (has(gsum)) check_like(*gsum, s, "the gradient of the sum");
+    c10::cuda::CUDAGuard guard(s.device());
+    const Tensor g = has(gy) ? gy->contiguous() : Tensor(), gs = has(gsum) ? gsum->contiguous() : Tensor();
+    int64_t sp = 0;
+    const Tensor sr = as_rows(s, sp);
+    Tensor ds = at::empty(s.sizes(), s.options()), dx, dw, db;
+    if (rate > 0) dx = at::empty(s.sizes(), s.options());
+    const auto popt = s.options().dtype(pdtype == MAM_F32 ? at::kFloat : s.scalar_type());
+    if (want_weight) dw = rows ? at::empty({width}, popt) : at::zeros({width}, popt);
+    if (want_bias) db = rows ? at::empty({width}, popt) : at::zeros({width}, popt);
+    if (rows) {
+        const size_t bytes = want_weight || want_bias ? mam_layer_norm_bwd_workspace_bytes(rows, width) : 0;
+        Tensor ws;
+        if (bytes) ws = at::empty({(int64_t)bytes}, s.options().dtype(at::kByte));
+        check_status(mam_layer_norm_bwd(ptr(g), ptr(gs), ptr(sr), sp, stats.const_data_ptr<float>(), ptr(w), pdtype,
+                                        (float)rate, (uint64_t)seed, seed_ptr(seed_at), mut(ds), mut(dx), mut(dw),
+                                        mut(db), rows, width, dtype, mut(ws), bytes,
+                                        at::cuda::getCurrentCUDAStream().stream()),
+                     "mam_layer_norm_bwd");
+    }
+    const auto none = [&] { return at::empty({0}, s.options()); };
+    return {ds, dx.defined() ? dx : none(), dw.defined() ? dw : none(), db.defined() ? db : none()};
+}
+
+Tensor dropout_forward(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dtype = dtype_code(x, "x");
+    check_drop(x, rate, seed_at);
+    if (has(residual)) check_like(*residual, x, "residual");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Tensor xc = x.contiguous(), rc = has(residual) ? residual->contiguous() : Tensor();
+    Tensor y = at::empty(x.sizes(), x.options());
+    if (y.numel())
+        check_status(mam_dropout_add(ptr(xc), ptr(rc), mut(y), y.numel(), dtype, (float)rate, (uint64_t)seed,
+                                     seed_ptr(seed_at), at::cuda::getCurrentCUDAStream().stream()),
+                     "mam_dropout_add");
+    return y;
+}
+
+Tensor gelu_forward(const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dtype = dtype_code(x, "x");
+    check_drop(x, rate, seed_at);
+    c10::cuda::CUDAGuard guard(x.device());
+    const Tensor xc = x.contiguous();
+    Tensor y = at::empty(x.sizes(), x.options());
+    if (y.numel())
+        check_status(mam_gelu_fwd(ptr(xc), mut(y), y.numel(), dtype, (float)rate, (uint64_t)seed, seed_ptr(seed_at),
+                                  at::cuda::getCurrentCUDAStream().stream()),
+                     "mam_gelu_fwd");
+    return y;
+}
+
+Tensor gelu_backward(const Tensor& gy, const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
+    TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+    const int dtype = dtype_code(x, "x");
+    check_drop(x, rate, seed_at);
+    check_like(gy, x, "the gradient of y");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Tensor gc = gy.contiguous(), xc = x.contiguous();
+    Tensor dx = at::empty(x.sizes(), x.options());
+    if (dx.numel())
+        check_status(mam_gelu_bwd(ptr(gc), ptr(xc), mut(dx), dx.numel(), dtype, (float)rate, (uint64_t)seed,
+                                  seed_ptr(seed_at), at::cuda::getCurrentCUDAStream().stream()),
+                     "mam_gelu_bwd");
+    return dx;
+}
+
+// ---------------------------------------------------------------- differentiable operators
+
+// The operators above through the dispatcher, so that tracing with fake tensors reaches their shape functions.
+#define MAM_OP(name, fn)                                                                                          \
+    static const auto name =                                                                                      \
+        c10::Dispatcher::singleton().findSchemaOrThrow("mamtorch_b200::" #fn, "").typed<decltype(fn)>()
+
+template <class... Ts>
+bool wants_grad(const Ts&... ts) {
+    return at::GradMode::is_enabled() && ((ts.defined() && ts.requires_grad()) || ...);
+}
+Tensor plain(const OptTensor& t) { return has(t) ? *t : Tensor(); }
+
+// Gradients are not differentiable again: under create_graph they carry a node that says so when it is run.
+void once(variable_list& grads, bool graph) {
+    if (!graph) return;
+    for (auto& g : grads)
+        if (g.defined())
+            g = (*std::make_shared<torch::autograd::DelayedError>(
+                "mamtorch_b200: layer_norm, dropout and gelu are differentiable once", 1))(
+                {g.detach().requires_grad_(true)})[0];
+}
+
+struct NormFn : torch::autograd::Function<NormFn> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual,
+                                 const OptTensor& weight, const OptTensor& bias, const OptTensor& seed_at, double eps,
+                                 double rate, int64_t seed) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        MAM_OP(op, layer_norm_forward);
+        auto out = op.call(x, residual, weight, bias, eps, rate, seed, seed_at, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({has(residual) ? out[1] : x, out.back(), plain(weight), plain(seed_at)});
+        ctx->saved_data["rate"] = rate;
+        ctx->saved_data["seed"] = seed;
+        const Tensor param = has(weight) ? *weight : plain(bias);
+        ctx->saved_data["f32"] = param.defined() && param.scalar_type() == at::kFloat;
+        ctx->saved_data["given"] = (int64_t)(has(residual) | has(weight) << 1 | has(bias) << 2);
+        out.pop_back();
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const bool graph = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        const auto saved = ctx->get_saved_variables();
+        const int64_t given = ctx->saved_data["given"].toInt();
+        const bool add = given & 1;
+        // the node has an edge for each tensor that was given, in the order of the arguments
+        size_t edge = 0;
+        const auto wanted = [&](bool there) { return there && ctx->needs_input_grad(edge++); };
+        const bool want_x = wanted(true), want_res = wanted(add), want_w = wanted(given & 2), want_b = wanted(given & 4);
+        const double rate = ctx->saved_data["rate"].toDouble();
+        const Tensor gs = add ? g[1] : Tensor();
+        variable_list r(8);
+        if (!g[0].defined() && !gs.defined()) return r;
+        MAM_OP(op, layer_norm_backward);
+        auto d = op.call(opt(g[0]), opt(gs), saved[0], saved[1], opt(saved[2]), rate, ctx->saved_data["seed"].toInt(),
+                         opt(saved[3]), ctx->saved_data["f32"].toBool(), want_w, want_b);
+        if (want_x) r[0] = rate > 0 ? d[1] : d[0];
+        if (want_res) r[1] = d[0];
+        if (want_w) r[2] = d[2];
+        if (want_b) r[3] = d[3];
+        once(r, graph);
+        return r;
+    }
+};
+
+struct DropoutFn : torch::autograd::Function<DropoutFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& seed_at,
+                          double rate, int64_t seed) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        MAM_OP(op, dropout_forward);
+        ctx->save_for_backward({plain(seed_at)});
+        ctx->saved_data["add"] = has(residual);
+        ctx->saved_data["rate"] = rate;
+        ctx->saved_data["seed"] = seed;
+        return op.call(x, residual, rate, seed, seed_at);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const bool graph = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        const double rate = ctx->saved_data["rate"].toDouble();
+        variable_list r(5);
+        if (!g[0].defined()) return r;
+        if (ctx->needs_input_grad(0)) {
+            MAM_OP(op, dropout_forward);
+            r[0] = rate > 0 ? op.call(g[0], std::nullopt, rate, ctx->saved_data["seed"].toInt(),
+                                      opt(ctx->get_saved_variables()[0]))
+                            : g[0];
+        }
+        if (ctx->saved_data["add"].toBool() && ctx->needs_input_grad(1)) r[1] = g[0];
+        once(r, graph);
+        return r;
+    }
+};
+
+struct GeluFn : torch::autograd::Function<GeluFn> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& seed_at, double rate, int64_t seed) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        MAM_OP(op, gelu_forward);
+        ctx->save_for_backward({x, plain(seed_at)});
+        ctx->saved_data["rate"] = rate;
+        ctx->saved_data["seed"] = seed;
+        return op.call(x, rate, seed, seed_at);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const bool graph = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        variable_list r(4);
+        if (!g[0].defined() || !ctx->needs_input_grad(0)) return r;
+        const auto saved = ctx->get_saved_variables();
+        MAM_OP(op, gelu_backward);
+        r[0] = op.call(g[0], saved[0], ctx->saved_data["rate"].toDouble(), ctx->saved_data["seed"].toInt(), opt(saved[1]));
+        once(r, graph);
+        return r;
+    }
+};
+
+Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    if (wants_grad(x, plain(weight), plain(bias)))
+        return NormFn::apply(x, std::nullopt, weight, bias, std::nullopt, eps, 0.0, 0)[0];
+    MAM_OP(op, layer_norm_forward);
+    return op.call(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt, false)[0];
+}
+std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
+                                                  const OptTensor& bias, double eps, double rate, int64_t seed,
+                                                  const OptTensor& seed_at) {
+    if (wants_grad(x, residual, plain(weight), plain(bias))) {
+        auto out = NormFn::apply(x, residual, weight, bias, seed_at, eps, rate, seed);
+        return {out[0], out[1]};
+    }
+    MAM_OP(op, layer_norm_forward);
+    auto out = op.call(x, residual, weight, bias, eps, rate, seed, seed_at, false);
+    return {out[0], out[1]};
+}
+Tensor dropout(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
+    if (wants_grad(x, plain(residual))) return DropoutFn::apply(x, residual, seed_at, rate, seed);
+    MAM_OP(op, dropout_forward);
+    return op.call(x, residual, rate, seed, seed_at);
+}
+Tensor gelu(const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
+    if (wants_grad(x)) return GeluFn::apply(x, seed_at, rate, seed);
+    MAM_OP(op, gelu_forward);
+    return op.call(x, rate, seed, seed_at);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(mamtorch_b200, m) {
+    m.def("layer_norm_forward(Tensor x, Tensor? residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, int drop_seed, Tensor? drop_seed_at, bool want_stats) -> Tensor[]");
+    m.def("layer_norm_backward(Tensor? gy, Tensor? gsum, Tensor s, Tensor stats, Tensor? weight, float drop_rate, int drop_seed, Tensor? drop_seed_at, bool params_f32, bool want_weight, bool want_bias) -> Tensor[]");
+    m.def("dropout_forward(Tensor x, Tensor? residual, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("gelu_forward(Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("gelu_backward(Tensor gy, Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", &layer_norm);
+    m.def("dropout_add_layer_norm(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> (Tensor, Tensor)", &dropout_add_layer_norm);
+    m.def("dropout(Tensor x, Tensor? residual, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor", &dropout);
+    m.def("gelu(Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor", &gelu);
+}
+TORCH_LIBRARY_IMPL(mamtorch_b200, CUDA, m) {
+    m.impl("layer_norm_forward", &layer_norm_forward);
+    m.impl("layer_norm_backward", &layer_norm_backward);
+    m.impl("dropout_forward", &dropout_forward);
+    m.impl("gelu_forward", &gelu_forward);
+    m.impl("gelu_backward", &gelu_backward);
+}

@@ -160,6 +160,40 @@ def _(argmax, argmin, K):
     return [argmax.new_empty(shape), argmax.new_empty(shape)]
 
 
+@torch.library.register_fake("mamtorch_b200::layer_norm_forward")
+def _(x, residual, weight, bias, eps, drop_rate, drop_seed, drop_seed_at, want_stats):
+    out = [x.new_empty(x.shape)]
+    if residual is not None:
+        out.append(x.new_empty(x.shape))
+    if want_stats:
+        out.append(x.new_empty((x.numel() // x.size(-1), 2), dtype=torch.float))
+    return out
+
+
+@torch.library.register_fake("mamtorch_b200::layer_norm_backward")
+def _(gy, gsum, s, stats, weight, drop_rate, drop_seed, drop_seed_at, params_f32, want_weight, want_bias):
+    kind = torch.float if params_f32 else s.dtype
+    none = s.new_empty((0,))
+    return [s.new_empty(s.shape), s.new_empty(s.shape) if drop_rate > 0 else none,
+            s.new_empty((s.size(-1),), dtype=kind) if want_weight else none,
+            s.new_empty((s.size(-1),), dtype=kind) if want_bias else none]
+
+
+@torch.library.register_fake("mamtorch_b200::dropout_forward")
+def _(x, residual, drop_rate, drop_seed, drop_seed_at):
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("mamtorch_b200::gelu_forward")
+def _(x, drop_rate, drop_seed, drop_seed_at):
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("mamtorch_b200::gelu_backward")
+def _(gy, x, drop_rate, drop_seed, drop_seed_at):
+    return x.new_empty(x.shape)
+
+
 @torch.library.register_fake("mamtorch_b200::dense_nt")
 def _(a, w):
     torch._check(a.dim() == 2 and w.dim() == 2 and a.size(1) == w.size(1))
@@ -387,3 +421,51 @@ def selection_count_update_(count: Tensor, argmax: Tensor, argmin: Tensor, hits=
     +1 for every weight any row selected as min, both added to the same matrix."""
     hmax, hmin = hits if hits is not None else selection_hits(argmax, argmin, count.size(1))
     return _ops.selection_count_update_(count, hmax, hmin)
+
+
+# ---------------------------------------------------------------- between the MAM layers of a transformer block
+# fp32, fp16 or bf16 activations of any shape; every operator differentiates once.  `drop_seed` is a number, or a tensor of
+# one int64 on the activations' device, which the kernels read when they run: a captured graph replays with a new mask
+# after the tensor was advanced.  The backward reads it again, so it must not change between a forward and its backward
+# (autograd raises if it did).
+
+def _drop_args(rate: float, seed):
+    rate = float(rate)
+    if not 0.0 <= rate < 1.0:
+        raise ValueError(f"drop_rate must be in [0, 1), not {rate}")
+    if rate == 0.0:
+        return 0.0, 0, None
+    if seed is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a number drawn during a graph capture would repeat one mask at every replay: "
+                               "pass drop_seed, as a tensor for a mask of its own at each replay")
+        return rate, fresh_drop_seed(), None
+    if isinstance(seed, Tensor):
+        return rate, 0, seed
+    return rate, int(seed), None
+
+
+def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
+    """Layer norm over the last dimension.  Weight and bias are fp32 or have the dtype of x.  Rows that lie a constant
+    distance apart (a slice of the last dimension) are read in place."""
+    return _ops.layer_norm.default(x, weight, bias, eps)
+
+
+def dropout_add_layer_norm(x: Tensor, residual: Tensor, weight: Tensor | None = None, bias: Tensor | None = None,
+                           eps: float = 1e-5, drop_rate: float = 0.0, drop_seed=None):
+    """(y, s): s = residual + dropout(x), the residual stream behind a block, and y = layer_norm(s), the input of the next.
+    One pass forward and one backward; equal to `dropout(x, ..., residual)` followed by `layer_norm` bit for bit (the
+    norm reads s as it is stored)."""
+    return _ops.dropout_add_layer_norm.default(x, residual, weight, bias, eps, *_drop_args(drop_rate, drop_seed))
+
+
+def dropout(x: Tensor, drop_rate: float, drop_seed=None, residual: Tensor | None = None) -> Tensor:
+    """dropout(x), or residual + dropout(x), the mask formed from the seed forward and backward and never stored.  It
+    always drops (a training-time operator).  Its masks are not those of `weight_drop` and the MAM layers' output dropout:
+    it takes one 64-bit draw for two elements, they take one for each."""
+    return _ops.dropout.default(x, residual, *_drop_args(drop_rate, drop_seed))
+
+
+def gelu(x: Tensor, drop_rate: float = 0.0, drop_seed=None) -> Tensor:
+    """dropout(x * Phi(x)), Phi the integral of the normal distribution: the exact GELU, with the dropout behind it."""
+    return _ops.gelu.default(x, *_drop_args(drop_rate, drop_seed))
