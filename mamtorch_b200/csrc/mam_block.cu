@@ -30,87 +30,186 @@ int drop_args(float rate, uint64_t seed, const int64_t* seed_at, DropArgs* d) {
 }
 
 // ---- forward of the norm ----
-template <typename T, int VEC, int NV, bool ADD>
-void fwd_launch(const NormFwdParams& p, bool warp, int threads, cudaStream_t st) {
-    if (warp) mam_norm_fwd_kernel<T, VEC, NV, ADD, true><<<(unsigned)((p.rows + 3) / 4), 128, 0, st>>>(p);
-    else mam_norm_fwd_kernel<T, VEC, NV, ADD, false><<<(unsigned)p.rows, threads, 0, st>>>(p);
-}
-
-template <typename T, int VEC, bool ADD>
-void fwd_pick(const NormFwdParams& p, const DevInfo& d, cudaStream_t st) {
-    constexpr int E = VEC == 1 ? 4 : 1;            // vectors a thread: E, 2E, 4E, 8E
-    const long long vecs = (p.width + VEC - 1) / VEC;
-    // few rows: as many threads a row as it has vectors; many: a warp a row while it fits, else 4E vectors a thread
-    const bool few = p.rows < 4 * (long long)d.sms;
-    const bool warp = vecs <= 32 * E || (!few && vecs <= 32 * 8 * E);
-    long long per = warp ? (vecs + 31) / 32 : few ? (vecs + 1023) / 1024 : 4 * E;
-    if (!warp && vecs > 1024 * per) per = (vecs + 1023) / 1024;
-    if (per > 8 * E) {
-        mam_norm_fwd_wide_kernel<T, VEC, ADD><<<(unsigned)p.rows, 1024, 0, st>>>(p);
-        return;
+template <typename T, int NV, bool ADD, int MODE>
+void fwd_launch(const NormFwdParams& p, int lanes, int threads, cudaStream_t st) {
+    const auto grid = [&](int per) { return (unsigned)((p.rows + per - 1) / per); };
+    if (lanes == 32) {
+        mam_norm_fwd_kernel<T, NV, ADD, MODE, false, 32><<<grid(4), 128, 0, st>>>(p);
+    } else if (lanes) {
+        if constexpr (NV == 1) {
+            if (lanes == 8) mam_norm_fwd_kernel<T, 1, ADD, MODE, false, 8><<<grid(16), 128, 0, st>>>(p);
+            else mam_norm_fwd_kernel<T, 1, ADD, MODE, false, 16><<<grid(8), 128, 0, st>>>(p);
+        }
+    } else if constexpr (NV != 3 && NV != 6) {
+        mam_norm_fwd_kernel<T, NV, ADD, MODE, true, 32><<<(unsigned)p.rows, threads, 0, st>>>(p);
     }
-    const int nv = per <= E ? E : per <= 2 * E ? 2 * E : per <= 4 * E ? 4 * E : 8 * E;
-    const int threads = (int)(((vecs + nv - 1) / nv + 31) / 32 * 32);
-    if (nv == E) fwd_launch<T, VEC, E, ADD>(p, warp, threads, st);
-    else if (nv == 2 * E) fwd_launch<T, VEC, 2 * E, ADD>(p, warp, threads, st);
-    else if (nv == 4 * E) fwd_launch<T, VEC, 4 * E, ADD>(p, warp, threads, st);
-    else fwd_launch<T, VEC, 8 * E, ADD>(p, warp, threads, st);
+}
+template <typename T, int NV, bool ADD>
+void fwd_mode(const NormFwdParams& p, bool aligned, int lanes, int threads, cudaStream_t st) {
+    const bool full = p.width == (long long)(lanes ? lanes : threads) * NV * VEC<T>;
+    if (!aligned) fwd_launch<T, NV, ADD, RAGGED>(p, lanes, threads, st);
+    else if (full) fwd_launch<T, NV, ADD, FULL>(p, lanes, threads, st);
+    else fwd_launch<T, NV, ADD, ALIGNED>(p, lanes, threads, st);
 }
 
-template <typename T>
-void fwd_type(const NormFwdParams& p, bool vec, const DevInfo& d, cudaStream_t st) {
-    constexpr int V = 16 / sizeof(T);
-    if (p.residual) {
-        if (vec) fwd_pick<T, V, true>(p, d, st);
-        else fwd_pick<T, 1, true>(p, d, st);
+template <typename T, bool ADD>
+void fwd_pick(const NormFwdParams& p, bool aligned, const DevInfo& d, cudaStream_t st) {
+    const long long vecs = (p.width + VEC<T> - 1) / VEC<T>;
+    // few rows: as many threads a row as it has vectors; many: a warp or less a row while it fits, else eight or four
+    // vectors a thread
+    const bool few = p.rows < 4 * (long long)d.sms;
+    if (vecs <= 32) {
+        fwd_mode<T, 1, ADD>(p, aligned, vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32, 0, st);
+    } else if (!few && vecs <= 256) {
+        if (vecs <= 64) fwd_mode<T, 2, ADD>(p, aligned, 32, 0, st);
+        else if (vecs <= 96) fwd_mode<T, 3, ADD>(p, aligned, 32, 0, st);
+        else if (vecs <= 128) fwd_mode<T, 4, ADD>(p, aligned, 32, 0, st);
+        else if (vecs <= 192) fwd_mode<T, 6, ADD>(p, aligned, 32, 0, st);
+        else fwd_mode<T, 8, ADD>(p, aligned, 32, 0, st);
+    } else if (vecs <= 4096) {
+        const int nv = few ? (vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 8) : vecs % 256 == 0 || vecs > 2048 ? 8 : 4;
+        const int threads = (int)(((vecs + nv - 1) / nv + 31) / 32 * 32);
+        if (nv == 1) fwd_mode<T, 1, ADD>(p, aligned, 0, threads, st);
+        else if (nv == 2) fwd_mode<T, 2, ADD>(p, aligned, 0, threads, st);
+        else if (nv == 4) fwd_mode<T, 4, ADD>(p, aligned, 0, threads, st);
+        else fwd_mode<T, 8, ADD>(p, aligned, 0, threads, st);
+    } else if (aligned) {
+        mam_norm_fwd_wide_kernel<T, ADD, ALIGNED><<<(unsigned)p.rows, 1024, 0, st>>>(p);
     } else {
-        if (vec) fwd_pick<T, V, false>(p, d, st);
-        else fwd_pick<T, 1, false>(p, d, st);
+        mam_norm_fwd_wide_kernel<T, ADD, RAGGED><<<(unsigned)p.rows, 1024, 0, st>>>(p);
     }
 }
 
 // ---- backward of the norm ----
 struct BwdPlan {
-    bool wide;          // rows beyond what a CTA's registers hold: rows and columns in kernels of their own
-    int per;            // values a thread
-    int group, groups;  // threads a row, rows at a time in a CTA
-    long long parts;    // partial rows
+    enum { WIDE, REGISTERS, RING } kind;   // rows beyond a CTA's registers; the next row in registers; rows in shared memory
+    int per;                               // values a thread
+    int group, groups;                     // threads a row, rows at a time in a CTA
+    long long parts;                       // partial rows
 };
 
-BwdPlan bwd_plan(int64_t rows, int64_t width, int sms) {
+// shared memory beside the rows: the weight, the barriers, their alignment
+size_t ring_rest(int64_t width) { return (size_t)width * 4 + 15 * 4 * 8 + 256; }
+int ring_stages(int64_t width, int groups, int size, int tensors, const DevInfo& d) {
+    const size_t row = tensors * (size_t)width * size * groups, rest = ring_rest(width) + 1024;
+    const long long n = (long long)d.max_smem > (long long)rest ? (long long)((d.max_smem - rest) / row) : 0;
+    return (int)(n < 4 ? n : 4);
+}
+
+// Most partial rows of a backward: a CTA an SM, or the slabs of the wide form.
+long long bwd_parts(int64_t rows, int64_t width, int sms) {
+    if (width <= 8192) return rows < sms ? rows : sms;
+    const long long groups = (width + NORM_COLS - 1) / NORM_COLS;
+    const long long slabs = (8LL * sms + groups - 1) / groups, most = (rows + 63) / 64;
+    return slabs < most ? slabs : most;
+}
+
+BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, const DevInfo& d) {
     BwdPlan b{};
-    b.wide = width > 8192;
-    if (b.wide) {
-        const long long groups = (width + NORM_COLS - 1) / NORM_COLS;
-        long long slabs = (8LL * sms + groups - 1) / groups;
-        const long long most = (rows + 63) / 64;
-        b.parts = slabs < most ? slabs : most;
+    if (width > 8192) {
+        b.kind = BwdPlan::WIDE;
+        b.parts = bwd_parts(rows, width, d.sms);
         return b;
     }
-    b.per = width <= 4096 ? 8 : 16;
-    b.group = (int)(((width + b.per - 1) / b.per + 31) / 32 * 32);
-    b.groups = 512 / b.group > 0 ? 512 / b.group : 1;
-    if (b.groups > 8) b.groups = 8;
-    const long long ctas = (rows + b.groups - 1) / b.groups, most = 2LL * sms;
-    b.parts = ctas < most ? ctas : most;
+    const auto threads = [&](int per) { return (int)(((width + per - 1) / per + 31) / 32 * 32); };
+    const int tensors = add ? 3 : 2;
+    if (aligned && width > 128) {
+        // The form that leaves the fewest threads without values: 8, 16 or 24 values a thread, of which an SM's registers
+        // hold 640, 512 and 384 threads.  Fewer values a thread cost more for what each row takes beside them, and a row at
+        // a time leaves its reduction uncovered.  bf16, GB/s by values a thread, 8 / 16 / 24: width 512 4000 / 5170 / 4560,
+        // 768 2790 / 2900 / 3060, 2048 3170 / 4000 / 3910, 5120 4370 / 4580 / 3960 (with dropout 5100 / 4650 / 3940).
+        b.kind = BwdPlan::RING;
+        double best = 0;
+        for (int per : {16, 24, 8}) {
+            const int group = threads(per), most = per == 24 ? 384 : per == 8 ? 640 : 512;
+            int groups = most / group < 15 ? most / group : 15;      // named barriers
+            while (groups > 1 && ring_stages(width, groups, size, tensors, d) < 3) --groups;
+            if (groups == 0 || ring_stages(width, groups, size, tensors, d) < 2) continue;
+            const double score = (double)width * groups / ((double)per * most) * (per == 8 ? 0.85 : 1.0) * (groups > 1 ? 1.0 : 0.8);
+            if (score <= best) continue;
+            best = score;
+            b.per = per;
+            b.group = group;
+            b.groups = groups;
+        }
+    }
+    if (b.per == 0) {
+        b.kind = BwdPlan::REGISTERS;
+        b.per = width <= 2048 ? 8 : 16;
+        const int n = (int)((width + b.per - 1) / b.per);
+        b.group = n <= 8 ? 8 : n <= 16 ? 16 : threads(b.per);
+        b.groups = b.group < 32 ? 512 / 32 * (32 / b.group) : 512 / b.group < 15 ? 512 / b.group : 15;
+    }
+    if (b.group >= 32) {
+        // few rows: over all SMs first
+        const long long fair = (rows + d.sms - 1) / d.sms;
+        if (fair < b.groups) b.groups = (int)fair;
+    }
+    const long long ctas = (rows + b.groups - 1) / b.groups;
+    b.parts = ctas < d.sms ? ctas : d.sms;
     return b;
 }
 
-template <typename T, int VEC, int NV, bool ADD>
-int bwd_launch(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
-    const size_t smem = b.groups > 1 ? (size_t)p.width * 8 : 0;   // at most 16 KB: several groups share a CTA up to width 2048
-    mam_norm_bwd_kernel<T, VEC, NV, ADD><<<(unsigned)b.parts, b.group * b.groups, smem, st>>>(p, b.group);
-    MAM_CUDA(cudaGetLastError());
-    return MAM_OK;
+template <typename T, int NV, bool ADD>
+int ring_launch(const NormBwdParams& p, const BwdPlan& b, const DevInfo& d, cudaStream_t st) {
+    BwdRing r{};
+    r.group = b.group;
+    r.groups = b.groups;
+    r.row_bytes = (unsigned)(p.width * sizeof(T));
+    r.stages = ring_stages(p.width, b.groups, sizeof(T), ADD ? 3 : 2, d);
+    if (r.stages < 2) return MAM_ERR_UNSUPPORTED;
+    const size_t row = (ADD ? 3 : 2) * (size_t)r.row_bytes * b.groups;
+    r.weights_at = (unsigned)((row * r.stages + 127) / 128 * 128);
+    r.bars_at = (unsigned)(r.weights_at + (p.width * 4 + 15) / 16 * 16);
+    r.bytes = r.bars_at + b.groups * r.stages * 8;
+    const auto run = [&](auto kernel) -> int {
+        MAM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)r.bytes));
+        kernel<<<(unsigned)b.parts, b.group * b.groups, r.bytes, st>>>(p, r);
+        MAM_CUDA(cudaGetLastError());
+        return MAM_OK;
+    };
+    if (p.width == (long long)b.group * NV * VEC<T>) return run(mam_norm_bwd_ring_kernel<T, NV, ADD, FULL>);
+    return run(mam_norm_bwd_ring_kernel<T, NV, ADD, ALIGNED>);
 }
 
-template <typename T, int VEC, bool ADD>
-int bwd_pick(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
-    if (!b.wide) {
-        if (b.per == 8) return bwd_launch<T, VEC, 8 / VEC, ADD>(p, b, st);
-        return bwd_launch<T, VEC, 16 / VEC, ADD>(p, b, st);
+template <typename T, int NV, bool ADD, int MODE>
+int bwd_launch(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
+    const int rows = b.group < 32 ? b.group * b.groups / 32 : b.groups;
+    const size_t smem = rows > 1 ? (size_t)rows * 2 * (size_t)p.width * 4 : 0;
+    const auto run = [&](auto kernel) -> int {
+        if (smem > 40 * 1024)
+            MAM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kernel<<<(unsigned)b.parts, b.group * b.groups, smem, st>>>(p, b.group);
+        MAM_CUDA(cudaGetLastError());
+        return MAM_OK;
+    };
+    if constexpr (MODE == RAGGED) {
+        if (b.group >= 32) return run(mam_norm_bwd_kernel<T, NV, ADD, MODE, 32>);
     }
-    mam_norm_bwd_wide_kernel<T, VEC, ADD><<<(unsigned)p.rows, 1024, 0, st>>>(p);
+    if constexpr (NV * VEC<T> == 8) {
+        if (b.group == 8) return run(mam_norm_bwd_kernel<T, NV, ADD, MODE, 8>);
+        return run(mam_norm_bwd_kernel<T, NV, ADD, MODE, 16>);
+    }
+    return MAM_ERR_UNSUPPORTED;
+}
+template <typename T, int NV, bool ADD>
+int bwd_mode(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
+    if (b.kind == BwdPlan::RING) return ring_launch<T, NV, ADD>(p, b, d, st);
+    if constexpr (NV * VEC<T> != 24)
+        if (!aligned || b.group >= 32) return bwd_launch<T, NV, ADD, RAGGED>(p, b, st);
+    if constexpr (NV * VEC<T> == 8) return bwd_launch<T, NV, ADD, ALIGNED>(p, b, st);   // narrow rows
+    return MAM_ERR_UNSUPPORTED;
+}
+
+template <typename T, bool ADD>
+int bwd_pick(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
+    if (b.kind != BwdPlan::WIDE) {
+        if (b.per == 8) return bwd_mode<T, 8 / VEC<T>, ADD>(p, b, aligned, d, st);
+        if (b.per == 16) return bwd_mode<T, 16 / VEC<T>, ADD>(p, b, aligned, d, st);
+        return bwd_mode<T, 24 / VEC<T>, ADD>(p, b, aligned, d, st);
+    }
+    if (aligned) mam_norm_bwd_wide_kernel<T, ADD, ALIGNED><<<(unsigned)p.rows, 1024, 0, st>>>(p);
+    else mam_norm_bwd_wide_kernel<T, ADD, RAGGED><<<(unsigned)p.rows, 1024, 0, st>>>(p);
     if (p.partial) {
         const long long per = (p.rows + b.parts - 1) / b.parts;
         mam_norm_bwd_cols_kernel<T><<<dim3((unsigned)((p.width + NORM_COLS - 1) / NORM_COLS), (unsigned)b.parts),
@@ -121,45 +220,75 @@ int bwd_pick(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
 }
 
 template <typename T>
-int bwd_type(const NormBwdParams& p, const BwdPlan& b, bool vec, bool add, void* dweight, void* dbias, cudaStream_t st) {
-    constexpr int V = 16 / sizeof(T);
+int bwd_type(const NormBwdParams& p, const BwdPlan& b, bool vec, bool add, void* dweight, void* dbias, const DevInfo& d,
+             cudaStream_t st) {
     int e;
-    if (add) e = vec ? bwd_pick<T, V, true>(p, b, st) : bwd_pick<T, 1, true>(p, b, st);
-    else e = vec ? bwd_pick<T, V, false>(p, b, st) : bwd_pick<T, 1, false>(p, b, st);
+    if (add) e = bwd_pick<T, true>(p, b, vec, d, st);
+    else e = bwd_pick<T, false>(p, b, vec, d, st);
     if (e != MAM_OK || !p.partial) return e;
-    mam_norm_params_kernel<T><<<(unsigned)((2 * p.width + NORM_COLS - 1) / NORM_COLS), NORM_COLS * NORM_LANES, 0, st>>>(
-        p.partial, dweight, dbias, b.parts, p.width, p.params_f32);
-    MAM_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((2 * p.width + NORM_COLS - 1) / NORM_COLS));
+    cfg.blockDim = dim3(NORM_COLS * NORM_LANES);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MAM_CUDA(cudaLaunchKernelEx(&cfg, mam_norm_params_kernel<T>, (const float*)p.partial, dweight, dbias, (long long)b.parts,
+                                p.width, p.params_f32));
     return MAM_OK;
 }
 
 // ---- pointwise ----
-template <typename T, int VEC, int OP>
-int point_launch(const PointParams& p, cudaStream_t st) {
-    constexpr int NV = VEC == 1 ? 4 : 2;
-    const long long blocks = (p.n + 256LL * VEC * NV - 1) / (256LL * VEC * NV);
+constexpr long long POINT_SPLIT = 1 << 18;   // elements from which a second launch costs less than ragged loads and stores
+template <typename T, int NV, int OP>
+int point_run(const PointParams& p, bool whole, cudaStream_t st) {
+    const long long per = (long long)POINT_THREADS * VEC<T> * NV, blocks = (p.n + per - 1) / per;
     if (blocks > 2147483647LL) return MAM_ERR_UNSUPPORTED;
-    mam_point_kernel<T, VEC, NV, OP><<<(unsigned)blocks, 256, 0, st>>>(p);
+    if (whole) mam_point_kernel<T, NV, OP, ALIGNED><<<(unsigned)blocks, POINT_THREADS, 0, st>>>(p);
+    else mam_point_kernel<T, NV, OP, RAGGED><<<(unsigned)blocks, POINT_THREADS, 0, st>>>(p);
     MAM_CUDA(cudaGetLastError());
     return MAM_OK;
+}
+template <typename T, int OP>
+int point_launch(const PointParams& p, bool aligned, const DevInfo& d, cudaStream_t st) {
+    const long long tail = p.n % VEC<T>;
+    if (aligned && tail && p.n > POINT_SPLIT) {
+        // whole vectors, and a second launch for the rest
+        PointParams q = p;
+        q.n = p.n - tail;
+        int e = point_launch<T, OP>(q, true, d, st);
+        if (e != MAM_OK) return e;
+        const long long whole = q.n;
+        q.x = static_cast<const T*>(p.x) + whole;
+        q.other = p.other ? static_cast<const T*>(p.other) + whole : nullptr;
+        q.out = static_cast<T*>(p.out) + whole;
+        q.first = p.first + whole;
+        q.n = tail;
+        return point_run<T, 1, OP>(q, false, st);
+    }
+    // four vectors a thread, or one where that leaves SMs without work
+    if (p.n > 4LL * POINT_THREADS * VEC<T> * 2 * d.sms) return point_run<T, 4, OP>(p, aligned && !tail, st);
+    return point_run<T, 1, OP>(p, aligned && !tail, st);
 }
 template <int OP>
 int point(const void* x, const void* other, void* out, int64_t n, int dtype, float rate, uint64_t seed,
           const int64_t* seed_at, void* stream) {
     if (bad_ptr(x) || bad_ptr(out) || n <= 0 || !dtype_ok(dtype)) return MAM_ERR_INVALID_ARGUMENT;
     if (!natural(x, dtype) || !natural(other, dtype) || !natural(out, dtype)) return MAM_ERR_INVALID_ARGUMENT;
-    PointParams p{x, other, out, n, {}};
+    PointParams p{x, other, out, n, 0, {}};
     int st = drop_args(rate, seed, seed_at, &p.drop);
     if (st != MAM_OK) return st;
     const DevInfo* d = nullptr;
     st = device_info(&d);
     if (st != MAM_OK) return st;
-    const bool vec = aligned16(x) && aligned16(other) && aligned16(out);
+    const bool aligned = aligned16(x) && aligned16(other) && aligned16(out);
     cudaStream_t cs = (cudaStream_t)stream;
     switch (dtype) {
-        case MAM_F32: return vec ? point_launch<float, 4, OP>(p, cs) : point_launch<float, 1, OP>(p, cs);
-        case MAM_F16: return vec ? point_launch<__half, 8, OP>(p, cs) : point_launch<__half, 1, OP>(p, cs);
-        default: return vec ? point_launch<__nv_bfloat16, 8, OP>(p, cs) : point_launch<__nv_bfloat16, 1, OP>(p, cs);
+        case MAM_F32: return point_launch<float, OP>(p, aligned, *d, cs);
+        case MAM_F16: return point_launch<__half, OP>(p, aligned, *d, cs);
+        default: return point_launch<__nv_bfloat16, OP>(p, aligned, *d, cs);
     }
 }
 
@@ -195,9 +324,10 @@ int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int
                      aligned16(residual) && aligned16(y) && aligned16(sum) && aligned16(weight) && aligned16(bias);
     cudaStream_t cs = (cudaStream_t)stream;
     switch (dtype) {
-        case MAM_F32: fwd_type<float>(p, vec, *d, cs); break;
-        case MAM_F16: fwd_type<__half>(p, vec, *d, cs); break;
-        default: fwd_type<__nv_bfloat16>(p, vec, *d, cs);
+        case MAM_F32: residual ? fwd_pick<float, true>(p, vec, *d, cs) : fwd_pick<float, false>(p, vec, *d, cs); break;
+        case MAM_F16: residual ? fwd_pick<__half, true>(p, vec, *d, cs) : fwd_pick<__half, false>(p, vec, *d, cs); break;
+        default:
+            residual ? fwd_pick<__nv_bfloat16, true>(p, vec, *d, cs) : fwd_pick<__nv_bfloat16, false>(p, vec, *d, cs);
     }
     MAM_CUDA(cudaGetLastError());
     return MAM_OK;
@@ -207,7 +337,7 @@ size_t mam_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width) {
     if (rows <= 0 || width <= 0) return 0;
     const DevInfo* d = nullptr;
     const int sms = device_info(&d) == MAM_OK ? d->sms : 148;
-    return (size_t)bwd_plan(rows, width, sms).parts * 2 * (size_t)width * 4;
+    return (size_t)bwd_parts(rows, width, sms) * 2 * (size_t)width * 4;
 }
 
 int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t s_pitch, const float* stats,
@@ -226,28 +356,32 @@ int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t 
     if (rows > MOST_ROWS || width > MOST_WIDTH) return MAM_ERR_UNSUPPORTED;
     const bool want_params = dweight || dbias;
     NormBwdParams p{gy, gsum, s, reinterpret_cast<const float2*>(stats), weight, ds, dx, nullptr, rows, width, s_pitch,
-                    param_dtype == MAM_F32, {}};
+                    param_dtype == MAM_F32, nullptr, {}};
     int st = drop_args(drop_rate, drop_seed, drop_seed_at, &p.drop);
     if (st != MAM_OK) return st;
     const DevInfo* d = nullptr;
     st = device_info(&d);
     if (st != MAM_OK) return st;
-    const BwdPlan b = bwd_plan(rows, width, d->sms);
+    const int per = 16 / dtype_size(dtype);
+    const bool vec = width % per == 0 && s_pitch % per == 0 && aligned16(gy) && aligned16(gsum) && aligned16(s) &&
+                     aligned16(ds) && aligned16(dx) && aligned16(weight);
+    const bool add = gsum || dx;
+    const BwdPlan b = bwd_plan(rows, width, dtype_size(dtype), add, vec, *d);
+    if (b.kind == BwdPlan::RING) {
+        st = wait_flag(&p.wait_flag);
+        if (st != MAM_OK) return st;
+    }
     if (want_params) {
         if (bad_ptr(workspace) || workspace_bytes < (size_t)b.parts * 2 * (size_t)width * 4 ||
             (reinterpret_cast<uintptr_t>(workspace) & 255u))
             return MAM_ERR_WORKSPACE;
         p.partial = static_cast<float*>(workspace);
     }
-    const int per = 16 / dtype_size(dtype);
-    const bool vec = width % per == 0 && s_pitch % per == 0 && aligned16(gy) && aligned16(gsum) && aligned16(s) &&
-                     aligned16(ds) && aligned16(dx) && aligned16(weight);
-    const bool add = gsum || dx;
     cudaStream_t cs = (cudaStream_t)stream;
     switch (dtype) {
-        case MAM_F32: return bwd_type<float>(p, b, vec, add, dweight, dbias, cs);
-        case MAM_F16: return bwd_type<__half>(p, b, vec, add, dweight, dbias, cs);
-        default: return bwd_type<__nv_bfloat16>(p, b, vec, add, dweight, dbias, cs);
+        case MAM_F32: return bwd_type<float>(p, b, vec, add, dweight, dbias, *d, cs);
+        case MAM_F16: return bwd_type<__half>(p, b, vec, add, dweight, dbias, *d, cs);
+        default: return bwd_type<__nv_bfloat16>(p, b, vec, add, dweight, dbias, *d, cs);
     }
 }
 

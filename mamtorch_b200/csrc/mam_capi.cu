@@ -544,6 +544,11 @@ int launch_bwd_split(const float* a, const float* b, const float* grad, const in
 }
 }  // namespace
 
+int mamb200::wait_flag(int** flag) {
+    MAM_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(flag), g_wait_gave_up));
+    return MAM_OK;
+}
+
 extern "C" {
 
 const char* mam_status_str(int status) {

@@ -3,14 +3,19 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include "mam_vec.cuh"
+
 namespace mamb200 {
 
-// the splitmix64 mixing function on seed + counter * golden ratio
-__device__ __forceinline__ unsigned long long mam_drop_mix(unsigned long long seed, unsigned long long counter) {
-    unsigned long long z = seed + counter * 0x9E3779B97F4A7C15ull;
+// The splitmix64 generator: a mixing function on seed + counter * golden ratio.
+constexpr unsigned long long MAM_DROP_STEP = 0x9E3779B97F4A7C15ull;
+__device__ __forceinline__ unsigned long long mam_drop_finish(unsigned long long z) {
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
     return z ^ (z >> 31);
+}
+__device__ __forceinline__ unsigned long long mam_drop_mix(unsigned long long seed, unsigned long long counter) {
+    return mam_drop_finish(seed + counter * MAM_DROP_STEP);
 }
 
 // The keep / drop decision of element `idx` in the MAM forward's epilogue and in mam_drop_f32: one mix an element, its
@@ -33,21 +38,59 @@ struct DropArgs {
     }
 };
 
-// x[j] = kept ? x[j] * scale : 0 for the VEC elements from `idx` on; VEC > 1 needs an even idx.  A select, not a product:
-// what is dropped leaves nothing behind, an infinity or NaN neither.
-template <int VEC>
-__device__ __forceinline__ void mam_drop_vec(float (&x)[VEC], unsigned long long seed, unsigned long long idx,
-                                             unsigned threshold, float scale) {
-    if constexpr (VEC == 1) {
-        const unsigned long long z = mam_drop_mix(seed, idx >> 1);
-        const unsigned draw = (idx & 1) ? (unsigned)(z >> 32) : (unsigned)z;
-        x[0] = draw >= threshold ? __fmul_rn(x[0], scale) : 0.f;
-    } else {
+// where the mixes of the elements from `idx` on begin: the one of pair j is of start + j * MAM_DROP_STEP
+__device__ __forceinline__ unsigned long long mam_drop_start(unsigned long long seed, long long idx) {
+    return seed + ((unsigned long long)idx >> 1) * MAM_DROP_STEP;
+}
+// x = kept ? x * scale : 0 for N pairs of elements from `start` on; `odd`: the first of them is the odd element of its
+// pair.  A select, not a product: what is dropped leaves nothing behind, an infinity or NaN neither.
+//
+// In 16-bit tensors the mixes are what bounds it (shifts, xors, compares and selects share a pipe of half rate).  The last
+// step of the mix only flips the lowest bit of the high half, where its highest bit is set, and is left out there: up to
+// a threshold of 2^31 such a half is kept either way, and a higher threshold is even (the rate, a float from 1/2 on, is
+// a multiple of 2^-24), so that it does not tell the two apart.
+template <int N>
+__device__ __forceinline__ void mam_drop_pairs(float2 (&x)[N], unsigned long long start, bool odd, unsigned threshold,
+                                               float scale) {
+    const float2 sc = make_float2(scale, scale);
+    const auto draw = [&](int j, unsigned& lo, unsigned& hi) {
+        // the 64-bit steps of mam_drop_finish in 32-bit ones
+        const unsigned long long z = start + (unsigned long long)j * MAM_DROP_STEP;
+        unsigned l = (unsigned)z, h = (unsigned)(z >> 32);
+        const auto times = [&](unsigned cl, unsigned ch) {
+            const unsigned long long w = (unsigned long long)l * cl;
+            h = l * ch + (h * cl + (unsigned)(w >> 32));
+            l = (unsigned)w;
+        };
+        const auto fold = [&](int k) {
+            l ^= __funnelshift_r(l, h, k);
+            h ^= h >> k;
+        };
+        fold(30);
+        times(0x1CE4E5B9u, 0xBF58476Du);
+        fold(27);
+        times(0x133111EBu, 0x94D049BBu);
+        lo = l ^ __funnelshift_r(l, h, 31);
+        hi = h;
+    };
+    if (!odd) {
 #pragma unroll
-        for (int j = 0; j < VEC; j += 2) {
-            const unsigned long long z = mam_drop_mix(seed, (idx + j) >> 1);
-            x[j] = (unsigned)z >= threshold ? __fmul_rn(x[j], scale) : 0.f;
-            x[j + 1] = (unsigned)(z >> 32) >= threshold ? __fmul_rn(x[j + 1], scale) : 0.f;
+        for (int j = 0; j < N; ++j) {
+            unsigned lo, hi;
+            draw(j, lo, hi);
+            const float2 y = mul2(x[j], sc);
+            x[j] = make_float2(lo >= threshold ? y.x : 0.f, hi >= threshold ? y.y : 0.f);
+        }
+    } else {
+        unsigned lo, high;
+        draw(0, lo, high);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            unsigned hi;
+            draw(j + 1, lo, hi);
+            const float2 y = mul2(x[j], sc);
+            x[j] = make_float2(high >= threshold ? y.x : 0.f, lo >= threshold ? y.y : 0.f);
+            high = hi;
         }
     }
 }

@@ -39,6 +39,8 @@ inline int device_info(const DevInfo** out) {
     return d.major == 10 ? MAM_OK : MAM_ERR_NOT_SM100;
 }
 
+int wait_flag(int** flag);    // device address of the flag that kernels set when a bounded wait runs out (mam_capi.cu)
+
 inline int bad_ptr(const void* p) { return p == nullptr; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

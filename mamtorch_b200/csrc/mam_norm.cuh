@@ -12,6 +12,7 @@
 // mean first and the deviations from it second, so that a mean far from zero costs no digits.
 #pragma once
 #include "mam_drop.cuh"
+#include "mam_ptx.cuh"
 #include "mam_vec.cuh"
 
 namespace mamb200 {
@@ -41,370 +42,668 @@ struct NormBwdParams {
     float* partial;            // [blocks][2][width]: sums of gy h and of gy over the block's rows, or nullptr
     long long rows, width, s_pitch;
     bool params_f32;
+    int* wait_flag;            // set where a bounded wait ran out
     DropArgs drop;
 };
 
-// Sum of two values over a row's threads: the lanes of one warp, or all warps of the CTA.  `slot` is shared memory of
-// one float2 a warp, another one for each reduction that may still be read.
-template <bool WARP>
-__device__ __forceinline__ float2 row_sum(float a, float b, float2* slot) {
+// Sums over a row's threads: LANES neighbouring lanes (8, 16 or 32), and with CTA all its warps.  `slot` is shared memory of
+// one value a warp, another one for each reduction that may still be read.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float a) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(~0u, a, o);
-        b += __shfl_xor_sync(~0u, b, o);
+    for (int o = LANES / 2; o > 0; o >>= 1) a += __shfl_xor_sync(~0u, a, o);
+    return a;
+}
+// Two sums at once: the first exchange leaves a in one half of the lanes and b in the other, six shuffles instead of ten.
+template <int LANES>
+__device__ __forceinline__ float2 lane_sum2(float a, float b) {
+    const bool upper = threadIdx.x & (LANES / 2);
+    const float v = lane_sum<LANES / 2>((upper ? b : a) + __shfl_xor_sync(~0u, upper ? a : b, LANES / 2));
+    const float w = __shfl_xor_sync(~0u, v, LANES / 2);
+    return upper ? make_float2(w, v) : make_float2(v, w);
+}
+// MOST: as many warps as the CTA can have, 16 or 32
+template <bool CTA, int LANES, int MOST>
+__device__ __forceinline__ float row_sum(float a, float* slot) {
+    a = lane_sum<LANES>(a);
+    if constexpr (CTA) {
+        const int k = threadIdx.x & (MOST - 1);
+        if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = a;
+        __syncthreads();
+        a = lane_sum<MOST>(k < (int)(blockDim.x >> 5) ? slot[k] : 0.f);
     }
-    if constexpr (WARP) return make_float2(a, b);
-    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) slot[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    const float2 v = lane < warps ? slot[lane] : make_float2(0.f, 0.f);
-    a = v.x;
-    b = v.y;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(~0u, a, o);
-        b += __shfl_xor_sync(~0u, b, o);
+    return a;
+}
+template <bool CTA, int LANES, int MOST>
+__device__ __forceinline__ float2 row_sum2(float a, float b, float2* slot) {
+    float2 v = lane_sum2<LANES>(a, b);
+    if constexpr (CTA) {
+        const int k = threadIdx.x & (MOST - 1);
+        if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+        __syncthreads();
+        v = k < (int)(blockDim.x >> 5) ? slot[k] : make_float2(0.f, 0.f);
+        v = lane_sum2<MOST>(v.x, v.y);
     }
-    return make_float2(a, b);
+    return v;
 }
 
 // s = round(residual + drop(x)), each step rounded by itself
-template <typename T, int VEC>
-__device__ __forceinline__ void add_residual(const Pack<T, VEC>& px, const Pack<T, VEC>& pr, const DropArgs& d,
-                                             unsigned long long seed, unsigned long long idx, Pack<T, VEC>& ps) {
-    float x[VEC], r[VEC];
-    unpack(px, x);
-    unpack(pr, r);
-    if (d.on) mam_drop_vec<VEC>(x, seed, idx, d.threshold, d.scale);
+template <typename T>
+__device__ __forceinline__ uint4 add_residual(const uint4& qx, const uint4& qr, const DropArgs& d,
+                                              unsigned long long start, bool odd) {
+    Vals<T> x, r;
+    unpack<T>(qx, x);
+    unpack<T>(qr, r);
+    if (d.on) mam_drop_pairs<VEC<T> / 2>(x, start, odd, d.threshold, d.scale);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = __fadd_rn(r[j], x[j]);
-    ps = pack<T, VEC>(x);
+    for (int j = 0; j < VEC<T> / 2; ++j) x[j] = add2(r[j], x[j]);
+    return pack<T>(x);
 }
 
-// mean, and 1 / sqrt(variance + eps), of `width` values of which this thread holds v[NV][VEC] (live(i): vector i is inside)
-template <bool WARP, int NV, int VEC, class Live>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NV][VEC], Live live, long long width, float eps, float2* slot) {
-    float s = 0.f;
+template <typename T>
+__device__ __forceinline__ float2 total(const Vals<T>& v) {
+    float2 s = v[0];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (!live(i)) continue;
-        float t = 0.f;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) t += v[i][j];
-        s += t;
-    }
-    const float n = (float)width;
-    float mu = row_sum<WARP>(s, 0.f, slot).x / n;
-    float d1 = 0.f, d2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if (!live(i)) continue;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float d = v[i][j] - mu;
-            d1 += d;
-            d2 = fmaf(d, d, d2);
-        }
-    }
-    const float2 t = row_sum<WARP>(d1, d2, slot + 32);
-    // the deviations' own mean is what rounding left in mu: with it a row of equal values comes out as exactly zero
-    const float off = t.x / n;
-    const float var = fmaxf(t.y / n - off * off, 0.f);
-    return make_float2(mu + off, __frsqrt_rn(var + eps));
+    for (int j = 1; j < VEC<T> / 2; ++j) s = add2(s, v[j]);
+    return s;
 }
 
-// Rows of up to NV * VEC * threads values: one warp a row, or one CTA.
-template <typename T, int VEC, int NV, bool ADD, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 1024) mam_norm_fwd_kernel(const __grid_constant__ NormFwdParams p) {
+// (mu, r) from the mean `mu` of the first reduction and the sums d1 of the deviations from it, d2 of their squares.  The
+// deviations' own mean is what rounding left in mu: with it a row of equal values comes out as exactly zero.
+__device__ __forceinline__ float2 row_stats(float mu, float d1, float d2, float n, float eps, float& off) {
+    off = d1 * (1.f / n);
+    return make_float2(mu + off, rsqrtf(fmaxf(d2 * (1.f / n) - off * off, 0.f) + eps));
+}
+
+// Rows of up to NV vectors a thread, held in registers.  CTA: a CTA a row; else LANES lanes a row, 128 / LANES rows a CTA.
+template <typename T, int NV, bool ADD, int MODE, bool CTA, int LANES>
+__global__ void __launch_bounds__(!CTA ? 128 : NV <= 2 ? 1024 : 512)
+mam_norm_fwd_kernel(const __grid_constant__ NormFwdParams p) {
     __shared__ float2 slot[64];
-    const int t = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : blockDim.x;
-    const long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    if (WARP && row >= p.rows) return;
-    const int width = (int)p.width;
-    auto col = [&](int i) { return (i * nt + t) * VEC; };
-    auto live = [&](int i) { return col(i) < width; };
-    const T* x = static_cast<const T*>(p.x) + row * p.x_pitch;
-    float v[NV][VEC];
+    constexpr int V = VEC<T>, nt = LANES, MOST = NV <= 2 ? 32 : 16;
+    const int t = threadIdx.x & (LANES - 1);
+    const long long row = CTA ? (long long)blockIdx.x
+                              : (long long)blockIdx.x * (128 / LANES) + threadIdx.x / LANES;
+    const int width = CTA || row < p.rows ? (int)p.width : 0;    // no columns beyond the last row
+    const int first = CTA ? (int)(threadIdx.x >> 5) * NV * 32 * V + t * V : t * V;    // a warp's vectors follow one another
+    auto col = [&](int i) { return first + i * nt * V; };
+    auto count = [&](int i) { return MODE == FULL ? (CTA || width ? V : 0) : min(V, width - col(i)); };
+    uint4 carry = make_uint4(0u, 0u, 0u, 0u);
+    const T* x0 = static_cast<const T*>(p.x);
+    const RowSrc<T, MODE> x(x0, p.x_pitch, p.rows, p.width, x0 + row * p.x_pitch);
+    uint4 qx[NV];
+    float2 v[NV][V / 2];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (count(i) > 0) qx[i] = x.load(col(i), count(i));
     if constexpr (ADD) {
-        const T* r = static_cast<const T*>(p.residual) + row * p.res_pitch;
-        T* sum = static_cast<T*>(p.sum) + row * p.width;
-        const unsigned long long seed = p.drop.on ? p.drop.seed_now() : 0;
-        Pack<T, VEC> px[NV], pr[NV];
+        const T* r0 = static_cast<const T*>(p.residual);
+        const RowSrc<T, MODE> r(r0, p.res_pitch, p.rows, p.width, r0 + row * p.res_pitch);
+        const long long at = row * p.width + first;
+        const unsigned long long start = p.drop.on ? mam_drop_start(p.drop.seed_now(), at) : 0;
+        const bool odd = MODE == RAGGED && (at & 1);
+        uint4 qr[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live(i)) {
-                px[i] = load_pack<T, VEC>(x + col(i));
-                pr[i] = load_pack<T, VEC>(r + col(i));
-            }
+            if (count(i) > 0) qr[i] = r.load(col(i), count(i));
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (live(i)) {
-                Pack<T, VEC> ps;
-                add_residual(px[i], pr[i], p.drop, seed, (unsigned long long)(row * p.width + col(i)), ps);
-                *reinterpret_cast<Pack<T, VEC>*>(sum + col(i)) = ps;
-                unpack(ps, v[i]);
+        for (int i = 0; i < NV; ++i) {
+            uint4 qs = make_uint4(0u, 0u, 0u, 0u);
+            if (count(i) > 0) {
+                qs = add_residual<T>(qx[i], qr[i], p.drop, start + (unsigned long long)(i * nt * (V / 2)) * MAM_DROP_STEP, odd);
+                unpack<T>(qs, v[i]);
             }
+            store_vec<T, MODE>(static_cast<T*>(p.sum) + at + i * nt * V, qs, width - col(i), t, nt, i == 0, i == NV - 1, carry);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live(i)) load_f32<T, VEC>(x + col(i), v[i]);
+            if (count(i) > 0) unpack<T>(qx[i], v[i]);
     }
-    const float2 st = row_stats<WARP>(v, live, p.width, p.eps, slot);
-    if (p.stats && t == 0) p.stats[row] = st;
-    T* y = static_cast<T*>(p.y) + row * p.width;
+    float2 s = splat2(0.f), d1 = s, d2 = s;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        if (live(i)) {
-            float w[VEC], b[VEC];
-            load_param<T, VEC>(p.weight, p.params_f32, col(i), 1.f, w);
-            load_param<T, VEC>(p.bias, p.params_f32, col(i), 0.f, b);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) w[j] = fmaf((v[i][j] - st.x) * st.y, w[j], b[j]);
-            store_f32<T, VEC>(y + col(i), w);
+        if (count(i) > 0) {
+            if (MODE == RAGGED && count(i) < V) keep_first<T>(v[i], count(i));
+            s = add2(s, total<T>(v[i]));
         }
+    const float n = (float)p.width;
+    const float mu = row_sum<CTA, LANES, MOST>(sum2(s), reinterpret_cast<float*>(slot)) * (1.f / n);
+    const float2 minus = splat2(-mu);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (count(i) > 0) {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) v[i][j] = add2(v[i][j], minus);
+            if (MODE == RAGGED && count(i) < V) keep_first<T>(v[i], count(i));
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) d2 = fma2(v[i][j], v[i][j], d2);
+            d1 = add2(d1, total<T>(v[i]));
+        }
+    const float2 d = row_sum2<CTA, LANES, MOST>(sum2(d1), sum2(d2), slot + 32);
+    float off;
+    const float2 st = row_stats(mu, d.x, d.y, n, p.eps, off);
+    if (p.stats && first == 0 && width) p.stats[row] = st;
+    const float2 r2 = splat2(st.y), o2 = splat2(-off * st.y);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        if (count(i) > 0) {
+            float2 w[V / 2], b[V / 2];
+            load_param<T, MODE>(p.weight, p.params_f32, col(i), count(i), 1.f, w);
+            load_param<T, MODE>(p.bias, p.params_f32, col(i), count(i), 0.f, b);
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) w[j] = fma2(fma2(v[i][j], r2, o2), w[j], b[j]);
+            q = pack<T>(w);
+        }
+        store_vec<T, MODE>(static_cast<T*>(p.y) + row * p.width + col(i), q, width - col(i), t, nt, i == 0, i == NV - 1, carry);
+    }
 }
 
 // Rows of any width: one CTA a row, which reads it again for each of its steps (from L2 mostly).
-template <typename T, int VEC, bool ADD>
+template <typename T, bool ADD, int MODE>
 __global__ void __launch_bounds__(1024) mam_norm_fwd_wide_kernel(const __grid_constant__ NormFwdParams p) {
     __shared__ float2 slot[64];
-    const long long row = blockIdx.x, step = (long long)blockDim.x * VEC;
-    const long long c0 = (long long)threadIdx.x * VEC;
-    const T* src = static_cast<const T*>(p.x) + row * p.x_pitch;
-    float s = 0.f;
+    constexpr int V = VEC<T>;
+    const long long row = blockIdx.x, width = p.width, step = (long long)blockDim.x * V;
+    const long long first = (long long)(threadIdx.x & ~31) * V;     // the warp's columns begin here: a loop for all its lanes
+    const int lane = threadIdx.x & 31;
+    const T* x0 = static_cast<const T*>(p.x);
+    RowSrc<T, MODE> src(x0, p.x_pitch, p.rows, width, x0 + row * p.x_pitch);
+    uint4 none;
+    float2 s = splat2(0.f), d1 = s, d2 = s;
+    auto count = [&](long long c) { return (int)min((long long)V, width - c); };
     if constexpr (ADD) {
-        const T* r = static_cast<const T*>(p.residual) + row * p.res_pitch;
-        T* sum = static_cast<T*>(p.sum) + row * p.width;
+        const T* r0 = static_cast<const T*>(p.residual);
+        const RowSrc<T, MODE> r(r0, p.res_pitch, p.rows, width, r0 + row * p.res_pitch);
         const unsigned long long seed = p.drop.on ? p.drop.seed_now() : 0;
-        for (long long c = c0; c < p.width; c += step) {
-            Pack<T, VEC> ps;
-            float v[VEC];
-            add_residual(load_pack<T, VEC>(src + c), load_pack<T, VEC>(r + c), p.drop, seed,
-                         (unsigned long long)(row * p.width + c), ps);
-            *reinterpret_cast<Pack<T, VEC>*>(sum + c) = ps;
-            unpack(ps, v);
-            float q = 0.f;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) q += v[j];
-            s += q;
+        for (long long c0 = first; c0 < width; c0 += step) {
+            const long long c = c0 + lane * V, at = row * width + c;
+            uint4 qs = make_uint4(0u, 0u, 0u, 0u);
+            if (c < width) {
+                qs = add_residual<T>(src.template load<false>(c, count(c)), r.load(c, count(c)), p.drop, mam_drop_start(seed, at),
+                                     MODE == RAGGED && (at & 1));
+                Vals<T> v;
+                unpack<T>(qs, v);
+                if (MODE == RAGGED && count(c) < V) keep_first<T>(v, count(c));
+                s = add2(s, total<T>(v));
+            }
+            store_vec<T, MODE>(static_cast<T*>(p.sum) + at, qs, (int)min(width - c, (long long)2 * V), lane, 32, true, true,
+                               none);
         }
-        src = sum;   // each thread reads back what it wrote itself
+        // read back behind the reduction's barrier
+        const T* s0 = static_cast<const T*>(p.sum);
+        src = RowSrc<T, MODE>(s0, width, p.rows, width, s0 + row * width);
     } else {
-        for (long long c = c0; c < p.width; c += step) {
-            float v[VEC], q = 0.f;
-            load_f32<T, VEC>(src + c, v);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) q += v[j];
-            s += q;
+        for (long long c = first + lane * V; c < width; c += step) {
+            Vals<T> v;
+            unpack<T>(src.template load<false>(c, count(c)), v);
+            if (MODE == RAGGED && count(c) < V) keep_first<T>(v, count(c));
+            s = add2(s, total<T>(v));
         }
     }
-    const float n = (float)p.width;
-    const float mu = row_sum<false>(s, 0.f, slot).x / n;
-    float d1 = 0.f, d2 = 0.f;
-    for (long long c = c0; c < p.width; c += step) {
-        float v[VEC], q1 = 0.f, q2 = 0.f;
-        load_f32<T, VEC>(src + c, v);
+    const float n = (float)width;
+    const float mu = row_sum<true, 32, 32>(sum2(s), reinterpret_cast<float*>(slot)) * (1.f / n);
+    const float2 minus = splat2(-mu);
+    for (long long c = first + lane * V; c < width; c += step) {
+        Vals<T> v;
+        unpack<T>(src.template load<false>(c, count(c)), v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float d = v[j] - mu;
-            q1 += d;
-            q2 = fmaf(d, d, q2);
-        }
-        d1 += q1;
-        d2 += q2;
+        for (int j = 0; j < V / 2; ++j) v[j] = add2(v[j], minus);
+        if (MODE == RAGGED && count(c) < V) keep_first<T>(v, count(c));
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) d2 = fma2(v[j], v[j], d2);
+        d1 = add2(d1, total<T>(v));
     }
-    const float2 t = row_sum<false>(d1, d2, slot + 32);
-    const float off = t.x / n;
-    const float2 st = make_float2(mu + off, __frsqrt_rn(fmaxf(t.y / n - off * off, 0.f) + p.eps));
+    const float2 d = row_sum2<true, 32, 32>(sum2(d1), sum2(d2), slot + 32);
+    float off;
+    const float2 st = row_stats(mu, d.x, d.y, n, p.eps, off);
     if (p.stats && threadIdx.x == 0) p.stats[row] = st;
-    T* y = static_cast<T*>(p.y) + row * p.width;
-    for (long long c = c0; c < p.width; c += step) {
-        float v[VEC], w[VEC], b[VEC];
-        load_f32<T, VEC>(src + c, v);
-        load_param<T, VEC>(p.weight, p.params_f32, c, 1.f, w);
-        load_param<T, VEC>(p.bias, p.params_f32, c, 0.f, b);
+    const float2 r2 = splat2(st.y), o2 = splat2(-off * st.y);
+    for (long long c0 = first; c0 < width; c0 += step) {
+        const long long c = c0 + lane * V;
+        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        if (c < width) {
+            Vals<T> v, w, b;
+            unpack<T>(src.template load<false>(c, count(c)), v);
+            load_param<T, MODE>(p.weight, p.params_f32, (int)c, count(c), 1.f, w);
+            load_param<T, MODE>(p.bias, p.params_f32, (int)c, count(c), 0.f, b);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) w[j] = fmaf((v[j] - st.x) * st.y, w[j], b[j]);
-        store_f32<T, VEC>(y + c, w);
+            for (int j = 0; j < V / 2; ++j) w[j] = fma2(fma2(add2(v[j], minus), r2, o2), w[j], b[j]);
+            q = pack<T>(w);
+        }
+        store_vec<T, MODE>(static_cast<T*>(p.y) + row * width + c, q, (int)min(width - c, (long long)2 * V), lane, 32, true, true,
+                           none);
     }
 }
 
-// Backward of rows of up to NV * VEC * group values.  blockDim.x / group groups of `group` threads (a multiple of 32)
+// Backward of rows of up to NV vectors a thread.  blockDim.x / group groups of `group` threads (8, 16 or a multiple of 32)
 // walk the rows; a thread keeps its columns' sums of gy h and gy in registers over all of them, and the CTA leaves one
-// partial row of each.
-template <typename T, int VEC, int NV, bool ADD>
-__global__ void __launch_bounds__(1024) mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
-    extern __shared__ float cols[];    // [2][width], with several groups
+// partial row of each.  The next row's vectors are on their way while a row is reduced.
+template <typename T, int NV, bool ADD, int MODE, int LANES>
+__global__ void __launch_bounds__(512)
+mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
+    extern __shared__ float cols[];    // [groups][2][width] at the end
     __shared__ float2 slot[2][32];
+    constexpr int V = VEC<T>, nt = LANES, MOST = 16;    // warps a CTA can have
+    if (LANES < 32) group = LANES;
     const int groups = blockDim.x / group, g = threadIdx.x / group, t = threadIdx.x % group;
-    const int warps = group >> 5, lane = threadIdx.x & 31, first = (g * group) >> 5;
+    const int lane = threadIdx.x & 31, tl = t & (nt - 1);
+    const int warps = group >> 5, slot0 = (g * group) >> 5;
     const int width = (int)p.width;
-    auto col = [&](int i) { return (i * group + t) * VEC; };
-    auto live = [&](int i) { return col(i) < width; };
-    const unsigned long long seed = ADD && p.drop.on ? p.drop.seed_now() : 0;
-    float w[NV][VEC], aw[NV][VEC], ab[NV][VEC];
+    const int first = (t >> 5) * NV * 32 * V + tl * V;    // a warp's vectors follow one another
+    auto col = [&](int i) { return first + i * nt * V; };
+    auto count = [&](int i) { return MODE == FULL ? V : min(V, width - col(i)); };
+    uint4 carry = make_uint4(0u, 0u, 0u, 0u), carry2 = carry;
+    float2 w[NV][V / 2], aw[NV][V / 2], ab[NV][V / 2];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (live(i)) load_param<T, VEC>(p.weight, p.params_f32, col(i), 1.f, w[i]);
+        if (count(i) > 0) load_param<T, MODE>(p.weight, p.params_f32, col(i), count(i), 1.f, w[i]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) aw[i][j] = ab[i][j] = 0.f;
+        for (int j = 0; j < V / 2; ++j) aw[i][j] = ab[i][j] = splat2(0.f);
     }
     const float inv_n = 1.f / (float)p.width;
+    // groups of less than a warp keep step with their warp
+    const int g0 = LANES < 32 ? (threadIdx.x >> 5) * (32 / LANES) : g;
     const long long step = (long long)gridDim.x * groups;
+    const bool has_gy = p.gy != nullptr, has_gs = ADD && p.gs != nullptr, has_dx = ADD && p.dx != nullptr;
+    const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy), *gs0 = static_cast<const T*>(p.gs);
+    // the row that is fetched: its pointer into s, its place in the contiguous tensors
+    long long base = (long long)blockIdx.x * groups + g0, ahead = base + (g - g0), at = ahead * p.width;
+    const T* ps = s0 + ahead * p.s_pitch;
+    const long long s_step = step * p.s_pitch, at_step = step * p.width;
+    const unsigned long long seed = has_dx ? p.drop.seed_now() : 0, drop_step = (unsigned long long)(at_step >> 1) * MAM_DROP_STEP;
+    unsigned long long start = mam_drop_start(seed, at + first);
+    uint4 qs[NV], qg[NV];
+    float2 st = make_float2(0.f, 0.f);
+    auto fetch = [&]() {
+        if (ahead >= p.rows) return;
+        const RowSrc<T, MODE> s(s0, p.s_pitch, p.rows, p.width, ps), y(gy0, p.width, p.rows, p.width, gy0 + at);
+        st = p.stats[ahead];
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (count(i) > 0) qs[i] = s.load(col(i), count(i));
+        if (has_gy)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (count(i) > 0) qg[i] = y.load(col(i), count(i));
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) qg[i] = make_uint4(0u, 0u, 0u, 0u);
+    fetch();
     int parity = 0;
-    for (long long row = (long long)blockIdx.x * groups + g; row < p.rows; row += step) {
-        const T* s = static_cast<const T*>(p.s) + row * p.s_pitch;
-        const float2 st = p.stats[row];
-        float h[NV][VEC], a[NV][VEC];
-        float s1 = 0.f, s2 = 0.f;
+    for (; base < p.rows; base += step) {
+        const bool valid = LANES == 32 || ahead < p.rows;
+        const long long row_at = at;
+        const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
+        const float rstd = st.y;
+        float2 h[NV][V / 2], a[NV][V / 2];
+        uint4 ga[NV];
+        float2 s1 = splat2(0.f), s2 = s1;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live(i)) {
-                load_f32<T, VEC>(s + col(i), h[i]);
-                if (p.gy) load_f32<T, VEC>(static_cast<const T*>(p.gy) + row * p.width + col(i), a[i]);
-                else
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) a[i][j] = 0.f;
+            if (valid && count(i) > 0) {
+                unpack<T>(qs[i], h[i]);
+                unpack<T>(qg[i], a[i]);
             }
+        if (has_gs && valid) {
+            const RowSrc<T, MODE> z(gs0, p.width, p.rows, p.width, gs0 + row_at);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (count(i) > 0) ga[i] = z.load(col(i), count(i));
+        }
+        ahead += step;
+        at += at_step;
+        ps += s_step;
+        fetch();
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live(i)) {
+            if (valid && count(i) > 0) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    h[i][j] = (h[i][j] - st.x) * st.y;
-                    aw[i][j] = fmaf(a[i][j], h[i][j], aw[i][j]);
-                    ab[i][j] += a[i][j];
-                    a[i][j] *= w[i][j];
-                    s1 += a[i][j];
-                    s2 = fmaf(a[i][j], h[i][j], s2);
+                for (int j = 0; j < V / 2; ++j) h[i][j] = mul2(add2(h[i][j], minus), r2);
+                if (MODE == RAGGED && count(i) < V) {
+                    keep_first<T>(h[i], count(i));
+                    keep_first<T>(a[i], count(i));
+                }
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    aw[i][j] = fma2(a[i][j], h[i][j], aw[i][j]);
+                    ab[i][j] = add2(ab[i][j], a[i][j]);
+                    a[i][j] = mul2(a[i][j], w[i][j]);
+                    s1 = add2(s1, a[i][j]);
+                    s2 = fma2(a[i][j], h[i][j], s2);
                 }
             }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            s1 += __shfl_xor_sync(~0u, s1, o);
-            s2 += __shfl_xor_sync(~0u, s2, o);
-        }
-        if (warps > 1) {
+        float2 m = lane_sum2<LANES>(sum2(s1), sum2(s2));
+        if (LANES == 32 && warps > 1) {
             // two sets of slots in turn: a set is written again only behind the next row's barrier
-            if (lane == 0) slot[parity][threadIdx.x >> 5] = make_float2(s1, s2);
+            if (lane == 0) slot[parity][threadIdx.x >> 5] = m;
             asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
-            const float2 v = lane < warps ? slot[parity][first + lane] : make_float2(0.f, 0.f);
-            s1 = v.x;
-            s2 = v.y;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                s1 += __shfl_xor_sync(~0u, s1, o);
-                s2 += __shfl_xor_sync(~0u, s2, o);
-            }
+            const int k = lane & (MOST - 1);
+            m = k < warps ? slot[parity][slot0 + k] : make_float2(0.f, 0.f);
+            m = lane_sum2<MOST>(m.x, m.y);
             parity ^= 1;
         }
-        s1 *= inv_n;
-        s2 *= inv_n;
+        // ds = r a - (r mean(a) + h r mean(a h))
+        const float2 c1 = splat2(-rstd * (m.x * inv_n)), c2 = splat2(-rstd * (m.y * inv_n));
+        const bool odd = MODE == RAGGED && ((row_at + first) & 1);
+        if (MODE == RAGGED) start = mam_drop_start(seed, row_at + first);
+        T *ds = static_cast<T*>(p.ds) + row_at, *dx = static_cast<T*>(p.dx) + row_at;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (live(i)) {
-                const long long at = row * p.width + col(i);
-                float d[VEC];
+        for (int i = 0; i < NV; ++i) {
+            const int rest = valid ? width - col(i) : 0;
+            uint4 q = make_uint4(0u, 0u, 0u, 0u), qd = q;
+            if (rest > 0) {
+                Vals<T> d;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) d[j] = st.y * (a[i][j] - s1 - h[i][j] * s2);
+                for (int j = 0; j < V / 2; ++j) d[j] = fma2(a[i][j], r2, fma2(h[i][j], c2, c1));
                 if constexpr (ADD) {
-                    if (p.gs) {
-                        float q[VEC];
-                        load_f32<T, VEC>(static_cast<const T*>(p.gs) + at, q);
+                    if (has_gs) {
+                        Vals<T> f;
+                        unpack<T>(ga[i], f);
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) d[j] += q[j];
+                        for (int j = 0; j < V / 2; ++j) d[j] = add2(d[j], f[j]);
                     }
                 }
-                store_f32<T, VEC>(static_cast<T*>(p.ds) + at, d);
+                q = pack<T>(d);
                 if constexpr (ADD) {
-                    if (p.dx) {
-                        mam_drop_vec<VEC>(d, seed, (unsigned long long)at, p.drop.threshold, p.drop.scale);
-                        store_f32<T, VEC>(static_cast<T*>(p.dx) + at, d);
+                    if (has_dx) {
+                        mam_drop_pairs<V / 2>(d, start + (unsigned long long)(i * nt * (V / 2)) * MAM_DROP_STEP, odd,
+                                              p.drop.threshold, p.drop.scale);
+                        qd = pack<T>(d);
                     }
                 }
             }
+            store_vec<T, MODE>(ds + col(i), q, rest, tl, nt, i == 0, i == NV - 1, carry);
+            if constexpr (ADD) {
+                if (has_dx) store_vec<T, MODE>(dx + col(i), qd, rest, tl, nt, i == 0, i == NV - 1, carry2);
+            }
+        }
+        start += drop_step;
     }
     if (!p.partial) return;
     float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
-    // the groups add to the columns one after the other: a fixed order
-    for (int k = 0; k < groups; ++k) {
-        if (g == k) {
+    // groups of one warp are added by shuffles, the rest in shared memory: a fixed order
+    const int rows = LANES < 32 ? (int)blockDim.x >> 5 : groups, mine = LANES < 32 ? (int)threadIdx.x >> 5 : g;
+    float* to = rows > 1 ? cols + (size_t)mine * 2 * width : out;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (live(i)) {
+    for (int i = 0; i < NV; ++i) {
+        float f[2][V];
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const int c = col(i) + j;
-                        if (k > 0) {
-                            aw[i][j] += cols[c];
-                            ab[i][j] += cols[width + c];
-                        }
-                        if (k < groups - 1) {
-                            cols[c] = aw[i][j];
-                            cols[width + c] = ab[i][j];
-                        } else {
-                            out[c] = aw[i][j];
-                            out[width + c] = ab[i][j];
-                        }
+        for (int j = 0; j < V / 2; ++j) {
+            split2(aw[i][j], f[0][2 * j], f[0][2 * j + 1]);
+            split2(ab[i][j], f[1][2 * j], f[1][2 * j + 1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if (LANES == 8) f[k][j] += __shfl_xor_sync(~0u, f[k][j], 8);
+                if (LANES < 32) f[k][j] += __shfl_xor_sync(~0u, f[k][j], 16);
+                if (col(i) + j < width && (LANES == 32 || lane < LANES)) to[k * width + col(i) + j] = f[k][j];
+            }
+    }
+    if (rows == 1) return;
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
+        float sum = cols[c];
+        for (int k = 1; k < rows; ++k) sum += cols[(size_t)k * 2 * width + c];
+        out[c] = sum;
+    }
+}
+
+// The same for aligned rows from a warp's width on, with the rows brought to shared memory by bulk copies: `stages` rows of
+// each group are there or on their way, whatever the registers leave room for.  With the next row's vectors in
+// registers instead, [16384, 5120] bf16 with dropout took 289 us and [32768, 4096] 336.
+// A row's stage is free when its group has passed the next row's barrier; thread 0 of the group then sends for the row
+// `stages - 1` ahead.
+struct BwdRing {
+    int group, groups, stages;
+    unsigned row_bytes;         // of one tensor's row
+    unsigned weights_at, bars_at, bytes;   // places in shared memory, and its size
+};
+
+template <typename T, int NV, bool ADD, int MODE>
+__global__ void __launch_bounds__(NV * VEC<T> == 8 ? 640 : NV * VEC<T> == 24 ? 384 : 512)
+mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_constant__ BwdRing ring) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float2 slot[2][32];
+    constexpr int V = VEC<T>, HALVES = V / 4, TENSORS = ADD ? 3 : 2, MOST = NV * V == 8 ? 32 : 16;      // warps a group can have
+    const int group = ring.group, groups = ring.groups, g = threadIdx.x / group, t = threadIdx.x - g * group;
+    const int lane = threadIdx.x & 31, warps = group >> 5, slot0 = (g * group) >> 5;
+    const int width = (int)p.width;
+    const int vec0 = (t >> 5) * NV * 32 + lane;     // a warp's vectors follow one another
+    auto col = [&](int i) { return (vec0 + i * 32) * V; };
+    auto live = [&](int i) { return MODE == FULL || col(i) < width; };
+    const bool has_gy = p.gy != nullptr, has_gs = ADD && p.gs != nullptr, has_dx = ADD && p.dx != nullptr;
+    const int tensors = 1 + has_gy + has_gs;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring.bars_at) + g * ring.stages;
+    unsigned char* mine = smem + (size_t)g * ring.stages * TENSORS * ring.row_bytes;      // [stage][s, gy, gs][row]
+    // the weight in fp32, the halves of a vector of eight apart: a warp's 16-byte reads then meet no bank twice
+    float4* weights = reinterpret_cast<float4*>(smem + ring.weights_at);
+    const int vecs = (width + V - 1) / V;
+    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+        float2 w[V / 2];
+        load_param<T, ALIGNED>(p.weight, p.params_f32, v * V, V, 1.f, w);
+#pragma unroll
+        for (int k = 0; k < HALVES; ++k)
+            weights[k * vecs + v] = make_float4(w[2 * k].x, w[2 * k].y, w[2 * k + 1].x, w[2 * k + 1].y);
+    }
+    if (t == 0) {
+        for (int k = 0; k < ring.stages; ++k) mbar_init(full + k, 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+
+    const long long step = (long long)gridDim.x * groups;
+    const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy), *gs0 = static_cast<const T*>(p.gs);
+    auto send = [&](long long row, int stage) {
+        if (row >= p.rows) return;
+        unsigned char* to = mine + (size_t)stage * TENSORS * ring.row_bytes;
+        mbar_expect_tx(full + stage, tensors * ring.row_bytes);
+        bulk_load(to, s0 + row * p.s_pitch, ring.row_bytes, full + stage);
+        if (has_gy) bulk_load(to + ring.row_bytes, gy0 + row * p.width, ring.row_bytes, full + stage);
+        if (has_gs) bulk_load(to + 2 * ring.row_bytes, gs0 + row * p.width, ring.row_bytes, full + stage);
+    };
+    long long row = (long long)blockIdx.x * groups + g;
+    if (t == 0)
+        for (int k = 0; k < ring.stages - 1; ++k) send(row + k * step, k);
+
+    float2 aw[NV][V / 2], ab[NV][V / 2];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) aw[i][j] = ab[i][j] = splat2(0.f);
+    const float inv_n = 1.f / (float)p.width;
+    long long at = row * p.width;
+    const long long at_step = step * p.width;
+    const unsigned long long drop_step = (unsigned long long)(at_step >> 1) * MAM_DROP_STEP;
+    unsigned long long start = has_dx ? mam_drop_start(p.drop.seed_now(), at + vec0 * V) : 0;
+    float2 next = row < p.rows ? p.stats[row] : make_float2(0.f, 0.f);
+    int stage = 0;
+    unsigned phase = 0, parity = 0;
+    bool lost = false;
+    for (; row < p.rows; row += step, at += at_step, start += drop_step) {
+        const float2 st = next;
+        if (row + step < p.rows) next = p.stats[row + step];
+        const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
+        const unsigned char* from = mine + (size_t)stage * TENSORS * ring.row_bytes;
+        if (!mbar_wait_bounded(full + stage, phase, lost ? 1024 : 1u << 22)) {
+            lost = true;            // the results are void, but every barrier is still met and every copy waited for
+            *p.wait_flag = 1;
+        }
+        float2 h[NV][V / 2], a[NV][V / 2], s1 = splat2(0.f), s2 = s1;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (live(i)) {
+                const uint4* q = reinterpret_cast<const uint4*>(from) + vec0 + i * 32;
+                unpack<T>(*q, h[i]);
+                if (has_gy) {
+                    unpack<T>(*reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(q) + ring.row_bytes), a[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V / 2; ++j) a[i][j] = splat2(0.f);
+                }
+                float2 w[V / 2];
+#pragma unroll
+                for (int k = 0; k < HALVES; ++k) {
+                    const float4 f = weights[k * vecs + vec0 + i * 32];
+                    w[2 * k] = make_float2(f.x, f.y);
+                    w[2 * k + 1] = make_float2(f.z, f.w);
+                }
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    h[i][j] = mul2(add2(h[i][j], minus), r2);
+                    aw[i][j] = fma2(a[i][j], h[i][j], aw[i][j]);
+                    ab[i][j] = add2(ab[i][j], a[i][j]);
+                    a[i][j] = mul2(a[i][j], w[j]);
+                    s1 = add2(s1, a[i][j]);
+                    s2 = fma2(a[i][j], h[i][j], s2);
+                }
+            }
+        float2 m = lane_sum2<32>(sum2(s1), sum2(s2));
+        if (warps > 1) {
+            // two sets of slots in turn: a set is written again only behind the next row's barrier
+            if (lane == 0) slot[parity][threadIdx.x >> 5] = m;
+            asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
+        } else {
+            __syncwarp();
+        }
+        // all have left the row before this one: its stage takes the row stages - 1 ahead
+        if (t == 0) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
+        if (warps > 1) {
+            m = (lane & (MOST - 1)) < warps ? slot[parity][slot0 + (lane & (MOST - 1))] : make_float2(0.f, 0.f);
+            m = lane_sum2<MOST>(m.x, m.y);
+            parity ^= 1;
+        }
+        // ds = r a - (r mean(a) + h r mean(a h))
+        const float2 c1 = splat2(-st.y * (m.x * inv_n)), c2 = splat2(-st.y * (m.y * inv_n));
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (live(i)) {
+                Vals<T> d;
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) d[j] = fma2(a[i][j], r2, fma2(h[i][j], c2, c1));
+                if constexpr (ADD) {
+                    if (has_gs) {
+                        Vals<T> f;
+                        unpack<T>(*(reinterpret_cast<const uint4*>(from + 2 * ring.row_bytes) + vec0 + i * 32), f);
+#pragma unroll
+                        for (int j = 0; j < V / 2; ++j) d[j] = add2(d[j], f[j]);
                     }
                 }
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.ds) + at + col(i)) = pack<T>(d);
+                if constexpr (ADD) {
+                    if (has_dx) {
+                        mam_drop_pairs<V / 2>(d, start + (unsigned long long)(i * 32 * (V / 2)) * MAM_DROP_STEP, false,
+                                              p.drop.threshold, p.drop.scale);
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.dx) + at + col(i)) = pack<T>(d);
+                    }
+                }
+            }
+        if (++stage == ring.stages) {
+            stage = 0;
+            phase ^= 1;
         }
-        if (groups > 1) __syncthreads();
+    }
+    if (!p.partial) return;
+    float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
+    // the groups' sums meet in the ring's memory, where no copy is on its way any more: a fixed order
+    __syncthreads();
+    float* cols = reinterpret_cast<float*>(smem);
+    float* to = groups > 1 ? cols + (size_t)g * 2 * width : out;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live(i)) {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {
+                *reinterpret_cast<float2*>(to + col(i) + 2 * j) = aw[i][j];
+                *reinterpret_cast<float2*>(to + width + col(i) + 2 * j) = ab[i][j];
+            }
+        }
+    if (groups == 1) return;
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
+        float sum = cols[c];
+        for (int k = 1; k < groups; ++k) sum += cols[(size_t)k * 2 * width + c];
+        out[c] = sum;
     }
 }
 
 // Backward of rows of any width: gradients of the rows, one CTA a row, without the columns' sums.
-template <typename T, int VEC, bool ADD>
+template <typename T, bool ADD, int MODE>
 __global__ void __launch_bounds__(1024) mam_norm_bwd_wide_kernel(const __grid_constant__ NormBwdParams p) {
     __shared__ float2 slot[32];
-    const long long row = blockIdx.x, step = (long long)blockDim.x * VEC, c0 = (long long)threadIdx.x * VEC;
-    const T* s = static_cast<const T*>(p.s) + row * p.s_pitch;
-    const T* gy = p.gy ? static_cast<const T*>(p.gy) + row * p.width : nullptr;
+    constexpr int V = VEC<T>;
+    const long long row = blockIdx.x, width = p.width, step = (long long)blockDim.x * V;
+    const long long first = (long long)(threadIdx.x & ~31) * V;
+    const int lane = threadIdx.x & 31;
+    const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy), *gs0 = static_cast<const T*>(p.gs);
+    const RowSrc<T, MODE> s(s0, p.s_pitch, p.rows, width, s0 + row * p.s_pitch),
+        gy(gy0, width, p.rows, width, gy0 + row * width), gs(gs0, width, p.rows, width, gs0 + row * width);
+    uint4 none;
     const float2 st = p.stats[row];
+    const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
     const unsigned long long seed = ADD && p.drop.on ? p.drop.seed_now() : 0;
-    float s1 = 0.f, s2 = 0.f;
-    if (gy)
-        for (long long c = c0; c < p.width; c += step) {
-            float h[VEC], a[VEC], w[VEC], q1 = 0.f, q2 = 0.f;
-            load_f32<T, VEC>(s + c, h);
-            load_f32<T, VEC>(gy + c, a);
-            load_param<T, VEC>(p.weight, p.params_f32, c, 1.f, w);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                a[j] *= w[j];
-                q1 += a[j];
-                q2 = fmaf(a[j], (h[j] - st.x) * st.y, q2);
-            }
-            s1 += q1;
-            s2 += q2;
-        }
-    const float2 m = row_sum<false>(s1, s2, slot);
-    s1 = m.x / (float)p.width;
-    s2 = m.y / (float)p.width;
-    for (long long c = c0; c < p.width; c += step) {
-        const long long at = row * p.width + c;
-        float h[VEC], d[VEC], w[VEC];
-        load_f32<T, VEC>(s + c, h);
-        if (gy) load_f32<T, VEC>(gy + c, d);
+    auto count = [&](long long c) { return (int)min((long long)V, width - c); };
+    // normalised values and weighted gradients of the vector at c
+    auto get = [&](long long c, Vals<T>& h, Vals<T>& a) {
+        Vals<T> w;
+        unpack<T>(s.load(c, count(c)), h);
+        if (p.gy) unpack<T>(gy.load(c, count(c)), a);
         else
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) d[j] = 0.f;
-        load_param<T, VEC>(p.weight, p.params_f32, c, 1.f, w);
+            for (int j = 0; j < V / 2; ++j) a[j] = splat2(0.f);
+        load_param<T, MODE>(p.weight, p.params_f32, (int)c, count(c), 1.f, w);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) d[j] = st.y * (d[j] * w[j] - s1 - (h[j] - st.x) * st.y * s2);
-        if constexpr (ADD) {
-            if (p.gs) {
-                load_f32<T, VEC>(static_cast<const T*>(p.gs) + at, h);
+        for (int j = 0; j < V / 2; ++j) {
+            h[j] = mul2(add2(h[j], minus), r2);
+            a[j] = mul2(a[j], w[j]);
+        }
+        if (MODE == RAGGED && count(c) < V) {
+            keep_first<T>(h, count(c));
+            keep_first<T>(a, count(c));
+        }
+    };
+    float2 s1 = splat2(0.f), s2 = s1;
+    if (p.gy)
+        for (long long c = first + lane * V; c < width; c += step) {
+            Vals<T> h, a;
+            get(c, h, a);
+            s1 = add2(s1, total<T>(a));
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) d[j] += h[j];
+            for (int j = 0; j < V / 2; ++j) s2 = fma2(a[j], h[j], s2);
+        }
+    const float2 m = row_sum2<true, 32, 32>(sum2(s1), sum2(s2), slot);
+    const float2 c1 = splat2(-st.y * (m.x / (float)width)), c2 = splat2(-st.y * (m.y / (float)width));
+    for (long long c0 = first; c0 < width; c0 += step) {
+        const long long c = c0 + lane * V, at = row * width + c;
+        const int rest = (int)min(width - c, (long long)2 * V);
+        uint4 q = make_uint4(0u, 0u, 0u, 0u), qd = q;
+        if (rest > 0) {
+            Vals<T> h, a;
+            get(c, h, a);
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) a[j] = fma2(a[j], r2, fma2(h[j], c2, c1));
+            if constexpr (ADD) {
+                if (p.gs) {
+                    unpack<T>(gs.load(c, count(c)), h);
+#pragma unroll
+                    for (int j = 0; j < V / 2; ++j) a[j] = add2(a[j], h[j]);
+                }
+            }
+            q = pack<T>(a);
+            if constexpr (ADD) {
+                if (p.dx) {
+                    mam_drop_pairs<V / 2>(a, mam_drop_start(seed, at), MODE == RAGGED && (at & 1), p.drop.threshold,
+                                          p.drop.scale);
+                    qd = pack<T>(a);
+                }
             }
         }
-        store_f32<T, VEC>(static_cast<T*>(p.ds) + at, d);
+        store_vec<T, MODE>(static_cast<T*>(p.ds) + at, q, rest, lane, 32, true, true, none);
         if constexpr (ADD) {
-            if (p.dx) {
-                mam_drop_vec<VEC>(d, seed, (unsigned long long)at, p.drop.threshold, p.drop.scale);
-                store_f32<T, VEC>(static_cast<T*>(p.dx) + at, d);
-            }
+            if (p.dx) store_vec<T, MODE>(static_cast<T*>(p.dx) + at, qd, rest, lane, 32, true, true, none);
         }
     }
 }
@@ -441,26 +740,34 @@ mam_norm_bwd_cols_kernel(const __grid_constant__ NormBwdParams p, long long rows
     }
 }
 
-// dw and db: the partial rows added in a fixed order, rounded once to the parameters' type.
+// dw and db: the partial rows added in a fixed order, rounded once to the parameters' type.  Bound by the latency of its
+// loads: eight rows at a time in a CTA, eight of them in flight a thread.  It is launched while the kernel before it still
+// runs, and waits for that one's partial rows here.
 template <typename T>
 __global__ void __launch_bounds__(NORM_COLS * NORM_LANES)
-mam_norm_params_kernel(const float* __restrict__ partial, void* dweight, void* dbias, long long parts, long long width,
+mam_norm_params_kernel(const float* partial, void* dweight, void* dbias, long long parts, long long width,
                        bool params_f32) {
     __shared__ float part[NORM_LANES][NORM_COLS];
     const int c = threadIdx.x % NORM_COLS, l = threadIdx.x / NORM_COLS;
     const long long n = (long long)blockIdx.x * NORM_COLS + c;      // 0 .. 2 * width - 1: weight, then bias
-    float s = 0.f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (n < 2 * width)
-        for (long long m = l; m < parts; m += NORM_LANES) s += partial[m * 2 * width + n];
-    part[l][c] = s;
+        for (long long m = l; m < parts; m += 8 * NORM_LANES)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (m + i * NORM_LANES < parts) s[i] += __ldcg(partial + (m + i * NORM_LANES) * 2 * width + n);
+    part[l][c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     __syncthreads();
     if (l != 0 || n >= 2 * width) return;
-    for (int i = 1; i < NORM_LANES; ++i) s += part[i][c];
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NORM_LANES; ++i) v += part[i][c];
     void* out = n < width ? dweight : dbias;
     if (!out) return;
-    const long long at = n < width ? n : n - width;
-    if (params_f32) static_cast<float*>(out)[at] = s;
-    else static_cast<T*>(out)[at] = from_f32<T>(s);
+    const long long k = n < width ? n : n - width;
+    if (params_f32) static_cast<float*>(out)[k] = v;
+    else static_cast<T*>(out)[k] = from_f32<T>(v);
 }
 
 }  // namespace mamb200

@@ -15,71 +15,115 @@ struct PointParams {
     const void* other;     // residual (or nullptr), or the upstream gradient
     void* out;
     long long n;
+    long long first;       // the place of x[0] in the tensor, even: where its draws begin
     DropArgs drop;
 };
 
 enum PointOp { POINT_DROPOUT, POINT_GELU, POINT_GELU_BWD };
 
-__device__ __forceinline__ float gelu_cdf(float x) { return 0.5f * (1.f + erff(x * 0.70710678118654752f)); }
+// q = -erfc(a / sqrt(2)) / 2 and e = exp(-a^2 / 2) for a = min(|x|, 15), pairwise: the form of Abramowitz and Stegun, 7.1.26,
+// t P(t) e with t = 1 / (1 + 0.28 a), P with six coefficients of our own fit instead of five (largest error of the fit
+// 9.3e-9; in fp32 1.9e-7 at a = 0, where the roundings of the sum to 0.5 count, and 6.3e-8 for a q).  erff and expf took
+// 33 instructions an element and twice the time of the bytes in bf16; this takes a reciprocal, an exponential and the
+// rest in packed pairs.  15: beyond it q is zero in fp32; min.NaN passes a NaN on.
+__device__ __forceinline__ void normal_tail(float2 x, float2& a, float2& q, float2& e) {
+    float u, v;
+    split2(x, u, v);
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(u) : "f"(fabsf(u)), "f"(15.f));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(fabsf(v)), "f"(15.f));
+    a = make_float2(u, v);
+    split2(fma2(a, splat2(0.28f), splat2(1.f)), u, v);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(u));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v));
+    const float2 t = make_float2(u, v);
+    split2(mul2(mul2(a, a), splat2(-0.72134752044448170f)), u, v);    // -a^2 / 2 in base 2
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(u));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(v));
+    e = make_float2(u, v);
+    float2 s = fma2(splat2(0.105807796f), t, splat2(-0.389872253f));
+    s = fma2(s, t, splat2(0.23699066f));
+    s = fma2(s, t, splat2(-0.268907934f));
+    s = fma2(s, t, splat2(-0.0674976185f));
+    s = fma2(s, t, splat2(-0.116520643f));
+    q = mul2(mul2(s, t), e);
+}
+// x Phi(x) = max(x, 0) + |x| q: zero at minus infinity, its limit
+__device__ __forceinline__ float2 gelu2(float2 x) {
+    float2 a, q, e;
+    normal_tail(x, a, q, e);
+    float u, v;
+    split2(x, u, v);
+    return fma2(a, q, make_float2(fmaxf(u, 0.f), fmaxf(v, 0.f)));
+}
+__device__ __forceinline__ float flip(float u, float sign) {
+    return __uint_as_float(__float_as_uint(u) ^ (__float_as_uint(sign) & 0x80000000u));
+}
+// Phi(x) + x phi(x) = 1/2 + sign(x) (1/2 + q + a phi(a))
+__device__ __forceinline__ float2 gelu_slope2(float2 x) {
+    float2 a, q, e;
+    normal_tail(x, a, q, e);
+    float u, v, xu, xv;
+    split2(add2(fma2(mul2(a, splat2(0.39894228040143268f)), e, splat2(0.5f)), q), u, v);
+    split2(x, xu, xv);
+    return add2(make_float2(flip(u, xu), flip(v, xv)), splat2(0.5f));
+}
 
-template <int OP, int VEC>
-__device__ __forceinline__ void point_apply(float (&x)[VEC], const float (&o)[VEC], bool has_other, const DropArgs& d,
-                                            unsigned long long seed, unsigned long long idx) {
-    if constexpr (OP == POINT_DROPOUT) {
-        if (d.on) mam_drop_vec<VEC>(x, seed, idx, d.threshold, d.scale);
-        if (has_other) {
+template <int OP, int N>
+__device__ __forceinline__ void point_apply(float2 (&x)[N], const float2 (&o)[N], bool has_other, const DropArgs& d,
+                                            unsigned long long start) {
+    if constexpr (OP != POINT_DROPOUT) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) x[j] = __fadd_rn(o[j], x[j]);
-        }
-    } else if constexpr (OP == POINT_GELU) {
+        for (int j = 0; j < N; ++j) x[j] = OP == POINT_GELU ? gelu2(x[j]) : mul2(o[j], gelu_slope2(x[j]));
+    }
+    // in the backward the mask comes last: what the forward dropped gets a zero whatever its x was
+    if (d.on) mam_drop_pairs<N>(x, start, false, d.threshold, d.scale);
+    if (OP == POINT_DROPOUT && has_other) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) x[j] *= gelu_cdf(x[j]);
-        if (d.on) mam_drop_vec<VEC>(x, seed, idx, d.threshold, d.scale);
-    } else {
-        // the mask last: what the forward dropped gets a zero whatever its x was
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float slope = fmaf(x[j] * 0.39894228040143268f, expf(-0.5f * x[j] * x[j]), gelu_cdf(x[j]));
-            x[j] = o[j] * slope;
-        }
-        if (d.on) mam_drop_vec<VEC>(x, seed, idx, d.threshold, d.scale);
+        for (int j = 0; j < N; ++j) x[j] = add2(o[j], x[j]);
     }
 }
 
-// NV vectors a thread, all loads first; the ragged end element by element.
-template <typename T, int VEC, int NV, int OP>
-__global__ void __launch_bounds__(256) mam_point_kernel(const __grid_constant__ PointParams p) {
-    const T* x = static_cast<const T*>(p.x);
-    const T* o = static_cast<const T*>(p.other);
+constexpr int POINT_THREADS = 128;
+
+// NV vectors a thread, all loads first; a CTA a block (CTAs that walk over several blocks took a sixth fewer instructions and
+// a tenth longer: their loads wait for the stores before them).  ALIGNED: whole vectors only, n is a multiple of them.
+// RAGGED: any n and any alignment, with the loads and stores of ragged rows, the whole tensor being one row.
+template <typename T, int NV, int OP, int MODE>
+__global__ void __launch_bounds__(POINT_THREADS, 8) mam_point_kernel(const __grid_constant__ PointParams p) {
+    constexpr int V = VEC<T>;
+    const bool has = p.other != nullptr;
+    const RowSrc<T, MODE> x(static_cast<const T*>(p.x), 0, 1, p.n, static_cast<const T*>(p.x)),
+        o(static_cast<const T*>(p.other), 0, 1, p.n, static_cast<const T*>(p.other));
     T* out = static_cast<T*>(p.out);
-    const unsigned long long seed = p.drop.on ? p.drop.seed_now() : 0;
-    const bool has = o != nullptr;
-    const long long base = ((long long)blockIdx.x * NV * 256 + threadIdx.x) * VEC;
-    Pack<T, VEC> px[NV], po[NV];
+    // ragged, a warp's vectors follow one another
+    constexpr int STEP = MODE == RAGGED ? 32 * V : POINT_THREADS * V;
+    const long long base = MODE == RAGGED
+        ? (((long long)blockIdx.x * (POINT_THREADS / 32) + (threadIdx.x >> 5)) * (NV * 32) + (threadIdx.x & 31)) * V
+        : ((long long)blockIdx.x * NV * POINT_THREADS + threadIdx.x) * V;
+    const unsigned long long start = p.drop.on ? mam_drop_start(p.drop.seed_now(), p.first + base) : 0;
+    uint4 px[NV], po[NV], carry = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const long long at = base + (long long)i * 256 * VEC;
-        if (at + VEC <= p.n) {
-            px[i] = load_pack<T, VEC>(x + at);
-            if (has) po[i] = load_pack<T, VEC>(o + at);
+        const long long at = base + i * STEP;
+        if (at < p.n) {
+            const int n = MODE == RAGGED ? (int)min((long long)V, p.n - at) : V;
+            px[i] = x.template load<false>(at, n);
+            if (has) po[i] = o.template load<false>(at, n);
         }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const long long at = base + (long long)i * 256 * VEC;
-        if (at + VEC <= p.n) {
-            float f[VEC], q[VEC];
-            unpack(px[i], f);
-            if (has) unpack(po[i], q);
-            point_apply<OP, VEC>(f, q, has, p.drop, seed, (unsigned long long)at);
-            store_f32<T, VEC>(out + at, f);
-        } else if (VEC > 1) {
-            for (long long e = at; e < p.n && e < at + VEC; ++e) {
-                float f[1] = {to_f32(x[e])}, q[1] = {has ? to_f32(o[e]) : 0.f};
-                point_apply<OP, 1>(f, q, has, p.drop, seed, (unsigned long long)e);
-                out[e] = from_f32<T>(f[0]);
-            }
+        const long long at = base + i * STEP;
+        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        if (at < p.n) {
+            float2 f[V / 2], g[V / 2];
+            unpack<T>(px[i], f);
+            if (has) unpack<T>(po[i], g);
+            point_apply<OP>(f, g, has, p.drop, start + (unsigned long long)(i * (STEP / 2)) * MAM_DROP_STEP);
+            q = pack<T>(f);
         }
+        const int rest = MODE == RAGGED ? (int)max(min(p.n - at, 2LL * V), 0LL) : at < p.n ? V : 0;
+        store_vec<T, MODE>(out + at, q, rest, threadIdx.x & 31, 32, i == 0, i == NV - 1, carry);
     }
 }
 
