@@ -313,7 +313,7 @@ int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int
         return MAM_ERR_INVALID_ARGUMENT;
     if (rows > MOST_ROWS || width > MOST_WIDTH) return MAM_ERR_UNSUPPORTED;
     NormFwdParams p{x, residual, weight, bias, y, sum, reinterpret_cast<float2*>(stats), rows, width, x_pitch,
-                    residual_pitch, eps, param_dtype == MAM_F32, {}};
+                    residual_pitch, eps, 1.0f / (float)width, param_dtype == MAM_F32, {}};
     int st = drop_args(drop_rate, drop_seed, drop_seed_at, &p.drop);
     if (st != MAM_OK) return st;
     const DevInfo* d = nullptr;
@@ -356,7 +356,7 @@ int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t 
     if (rows > MOST_ROWS || width > MOST_WIDTH) return MAM_ERR_UNSUPPORTED;
     const bool want_params = dweight || dbias;
     NormBwdParams p{gy, gsum, s, reinterpret_cast<const float2*>(stats), weight, ds, dx, nullptr, rows, width, s_pitch,
-                    param_dtype == MAM_F32, nullptr, {}};
+                    1.0f / (float)width, param_dtype == MAM_F32, nullptr, {}};
     int st = drop_args(drop_rate, drop_seed, drop_seed_at, &p.drop);
     if (st != MAM_OK) return st;
     const DevInfo* d = nullptr;

@@ -26,7 +26,7 @@ struct NormFwdParams {
     void* sum;                 // s, with a residual
     float2* stats;             // (mu, r) of each row, or nullptr
     long long rows, width, x_pitch, res_pitch;
-    float eps;
+    float eps, inv_width;
     bool params_f32;
     DropArgs drop;
 };
@@ -41,6 +41,7 @@ struct NormBwdParams {
     void* dx;                  // drop(ds), or nullptr
     float* partial;            // [blocks][2][width]: sums of gy h and of gy over the block's rows, or nullptr
     long long rows, width, s_pitch;
+    float inv_width;
     bool params_f32;
     int* wait_flag;            // set where a bounded wait ran out
     DropArgs drop;
@@ -108,11 +109,13 @@ __device__ __forceinline__ float2 total(const Vals<T>& v) {
     return s;
 }
 
-// (mu, r) from the mean `mu` of the first reduction and the sums d1 of the deviations from it, d2 of their squares.  The
-// deviations' own mean is what rounding left in mu: with it a row of equal values comes out as exactly zero.
-__device__ __forceinline__ float2 row_stats(float mu, float d1, float d2, float n, float eps, float& off) {
-    off = d1 * (1.f / n);
-    return make_float2(mu + off, rsqrtf(fmaxf(d2 * (1.f / n) - off * off, 0.f) + eps));
+// (mean, r) from the mean `mu` of the first reduction and the sums d1 of the deviations from it and d2 of their squares.  The
+// deviations' own mean is what rounding left in mu; `off` is the step from mu to the corrected mean as it is stored, so
+// that deviation - off is s - mean, the same as in the backward, and zero for a row of equal values whatever r is.
+__device__ __forceinline__ float2 row_stats(float mu, float d1, float d2, float inv_n, float eps, float& off) {
+    const float mean = fmaf(d1, inv_n, mu);
+    off = mean - mu;
+    return make_float2(mean, rsqrtf(fmaxf(d2 * inv_n - off * (2.f * (d1 * inv_n) - off), 0.f) + eps));
 }
 
 // Rows of up to NV vectors a thread, held in registers.  CTA: a CTA a row; else LANES lanes a row, 128 / LANES rows a CTA.
@@ -167,8 +170,7 @@ mam_norm_fwd_kernel(const __grid_constant__ NormFwdParams p) {
             if (MODE == RAGGED && count(i) < V) keep_first<T>(v[i], count(i));
             s = add2(s, total<T>(v[i]));
         }
-    const float n = (float)p.width;
-    const float mu = row_sum<CTA, LANES, MOST>(sum2(s), reinterpret_cast<float*>(slot)) * (1.f / n);
+    const float mu = row_sum<CTA, LANES, MOST>(sum2(s), reinterpret_cast<float*>(slot)) * p.inv_width;
     const float2 minus = splat2(-mu);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -182,9 +184,9 @@ mam_norm_fwd_kernel(const __grid_constant__ NormFwdParams p) {
         }
     const float2 d = row_sum2<CTA, LANES, MOST>(sum2(d1), sum2(d2), slot + 32);
     float off;
-    const float2 st = row_stats(mu, d.x, d.y, n, p.eps, off);
+    const float2 st = row_stats(mu, d.x, d.y, p.inv_width, p.eps, off);
     if (p.stats && first == 0 && width) p.stats[row] = st;
-    const float2 r2 = splat2(st.y), o2 = splat2(-off * st.y);
+    const float2 r2 = splat2(st.y), o2 = splat2(-off);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         uint4 q = make_uint4(0u, 0u, 0u, 0u);
@@ -193,7 +195,7 @@ mam_norm_fwd_kernel(const __grid_constant__ NormFwdParams p) {
             load_param<T, MODE>(p.weight, p.params_f32, col(i), count(i), 1.f, w);
             load_param<T, MODE>(p.bias, p.params_f32, col(i), count(i), 0.f, b);
 #pragma unroll
-            for (int j = 0; j < V / 2; ++j) w[j] = fma2(fma2(v[i][j], r2, o2), w[j], b[j]);
+            for (int j = 0; j < V / 2; ++j) w[j] = fma2(mul2(add2(v[i][j], o2), r2), w[j], b[j]);
             q = pack<T>(w);
         }
         store_vec<T, MODE>(static_cast<T*>(p.y) + row * p.width + col(i), q, width - col(i), t, nt, i == 0, i == NV - 1, carry);
@@ -242,8 +244,7 @@ __global__ void __launch_bounds__(1024) mam_norm_fwd_wide_kernel(const __grid_co
             s = add2(s, total<T>(v));
         }
     }
-    const float n = (float)width;
-    const float mu = row_sum<true, 32, 32>(sum2(s), reinterpret_cast<float*>(slot)) * (1.f / n);
+    const float mu = row_sum<true, 32, 32>(sum2(s), reinterpret_cast<float*>(slot)) * p.inv_width;
     const float2 minus = splat2(-mu);
     for (long long c = first + lane * V; c < width; c += step) {
         Vals<T> v;
@@ -257,9 +258,9 @@ __global__ void __launch_bounds__(1024) mam_norm_fwd_wide_kernel(const __grid_co
     }
     const float2 d = row_sum2<true, 32, 32>(sum2(d1), sum2(d2), slot + 32);
     float off;
-    const float2 st = row_stats(mu, d.x, d.y, n, p.eps, off);
+    const float2 st = row_stats(mu, d.x, d.y, p.inv_width, p.eps, off);
     if (p.stats && threadIdx.x == 0) p.stats[row] = st;
-    const float2 r2 = splat2(st.y), o2 = splat2(-off * st.y);
+    const float2 r2 = splat2(st.y), o2 = splat2(-off);
     for (long long c0 = first; c0 < width; c0 += step) {
         const long long c = c0 + lane * V;
         uint4 q = make_uint4(0u, 0u, 0u, 0u);
@@ -269,7 +270,7 @@ __global__ void __launch_bounds__(1024) mam_norm_fwd_wide_kernel(const __grid_co
             load_param<T, MODE>(p.weight, p.params_f32, (int)c, count(c), 1.f, w);
             load_param<T, MODE>(p.bias, p.params_f32, (int)c, count(c), 0.f, b);
 #pragma unroll
-            for (int j = 0; j < V / 2; ++j) w[j] = fma2(fma2(add2(v[j], minus), r2, o2), w[j], b[j]);
+            for (int j = 0; j < V / 2; ++j) w[j] = fma2(mul2(add2(add2(v[j], minus), o2), r2), w[j], b[j]);
             q = pack<T>(w);
         }
         store_vec<T, MODE>(static_cast<T*>(p.y) + row * width + c, q, (int)min(width - c, (long long)2 * V), lane, 32, true, true,
@@ -302,7 +303,7 @@ mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) aw[i][j] = ab[i][j] = splat2(0.f);
     }
-    const float inv_n = 1.f / (float)p.width;
+    const float inv_n = p.inv_width;
     // groups of less than a warp keep step with their warp
     const int g0 = LANES < 32 ? (threadIdx.x >> 5) * (32 / LANES) : g;
     const long long step = (long long)gridDim.x * groups;
@@ -514,7 +515,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) aw[i][j] = ab[i][j] = splat2(0.f);
-    const float inv_n = 1.f / (float)p.width;
+    const float inv_n = p.inv_width;
     long long at = row * p.width;
     const long long at_step = step * p.width;
     const unsigned long long drop_step = (unsigned long long)(at_step >> 1) * MAM_DROP_STEP;
@@ -675,7 +676,7 @@ __global__ void __launch_bounds__(1024) mam_norm_bwd_wide_kernel(const __grid_co
             for (int j = 0; j < V / 2; ++j) s2 = fma2(a[j], h[j], s2);
         }
     const float2 m = row_sum2<true, 32, 32>(sum2(s1), sum2(s2), slot);
-    const float2 c1 = splat2(-st.y * (m.x / (float)width)), c2 = splat2(-st.y * (m.y / (float)width));
+    const float2 c1 = splat2(-st.y * (m.x * p.inv_width)), c2 = splat2(-st.y * (m.y * p.inv_width));
     for (long long c0 = first; c0 < width; c0 += step) {
         const long long c = c0 + lane * V, at = row * width + c;
         const int rest = (int)min(width - c, (long long)2 * V);

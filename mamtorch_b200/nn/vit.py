@@ -11,7 +11,12 @@ without the example's dependence on a checkpoint or a dataset:
   * `vcon_step_all`                            one schedule step for every MAM layer of a model;
   * `MAMMlpBlock`                              LayerNorm -> MAM(d, 4d) -> GELU -> MAM(4d, d) + residual,
                                                the MLP half of a ViT encoder layer, for runs on
-                                               synthetic tokens;
+                                               synthetic tokens; with `fused=True` what stands between
+                                               the MAM layers, dropout included, runs in this library's
+                                               own kernels;
+  * `MAMMlpStack`                              such blocks one after the other with the encoder's final
+                                               norm: each residual addition, its dropout and the norm of
+                                               the next block in one pass;
   * `GraphedStep`                              forward + backward of a module captured in one CUDA
                                                graph on static buffers (the kernels take the current
                                                stream and allocate through torch's caching allocator,
@@ -22,9 +27,11 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from . import functional as MF
 from .v4.fullyconnected import FullyConnected
 
-__all__ = ["mlp_dense_paths", "swap_linear_for_mam", "vcon_step_all", "mam_layers", "MAMMlpBlock", "GraphedStep"]
+__all__ = ["mlp_dense_paths", "swap_linear_for_mam", "vcon_step_all", "mam_layers", "MAMMlpBlock", "MAMMlpStack",
+           "GraphedStep"]
 
 
 def mlp_dense_paths(num_layers: int = 12, intermediate: bool = True, output: bool = True,
@@ -82,16 +89,40 @@ def vcon_step_all(model: nn.Module) -> None:
         layer.vcon_step()
 
 
+class _DropSeeds(nn.Module):
+    """Seeds for the dropout of a module.  Eagerly they are numbers from torch's CPU generator.  Inside a graph capture a
+    number would repeat one mask at every replay, so there a device counter is advanced and copied, which the graph does
+    again each time it runs."""
+
+    def __init__(self, device=None):
+        super().__init__()
+        self.register_buffer("counter", torch.tensor([MF.fresh_drop_seed()], dtype=torch.int64, device=device),
+                             persistent=False)
+
+    def forward(self):
+        if not (self.counter.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return MF.fresh_drop_seed()
+        self.counter.add_(0x632BE59BD9B4E019)
+        return self.counter.clone()
+
+
 class MAMMlpBlock(nn.Module):
     """The MLP half of a pre-norm transformer encoder layer with MAM dense layers:
     x + MAM_2(GELU(MAM_1(LayerNorm(x)))), shapes [..., hidden] -> [..., hidden].
 
-    ViT-B/16: hidden 768, intermediate 3072, 197 tokens per image."""
+    ViT-B/16: hidden 768, intermediate 3072, 197 tokens per image.
+
+    `fused=True` runs norm, GELU and residual in this library's kernels (equal to torch's up to rounding) and allows
+    `drop_rate`: dropout behind the GELU and before the residual, in training, with masks that are never stored."""
 
     def __init__(self, hidden: int = 768, intermediate: int = 3072, vcon_steps: int = 0, vcon_type: str = "linear",
                  store_args: bool = False, residual: bool = True, layer_norm_eps: float = 1e-12, device=None,
-                 dtype=None):
+                 dtype=None, fused: bool = False, drop_rate: float = 0.0):
         super().__init__()
+        if not 0.0 <= drop_rate < 1.0:
+            raise ValueError(f"drop_rate must be in [0, 1), not {drop_rate}")
+        if drop_rate > 0 and not fused:
+            raise ValueError("drop_rate needs fused=True")
         self.norm = nn.LayerNorm(hidden, eps=layer_norm_eps, device=device, dtype=dtype)
         self.fc1 = FullyConnected(hidden, intermediate, vcon_steps=vcon_steps, vcon_type=vcon_type,
                                   store_args=store_args, device=device, dtype=dtype)
@@ -99,14 +130,61 @@ class MAMMlpBlock(nn.Module):
         self.fc2 = FullyConnected(intermediate, hidden, vcon_steps=vcon_steps, vcon_type=vcon_type,
                                   store_args=store_args, device=device, dtype=dtype)
         self.residual = residual
+        self.fused = fused
+        self.drop_rate = drop_rate
+        self.drop_seeds = _DropSeeds(device) if drop_rate > 0 else None
+
+    def drop_args(self):
+        """(rate, seed) of the next dropout: nothing outside training."""
+        if self.drop_seeds is None or not self.training:
+            return 0.0, None
+        return self.drop_rate, self.drop_seeds()
+
+    def mlp(self, h: torch.Tensor) -> torch.Tensor:
+        """The MAM layers on a normalised input, with the fused activation between them."""
+        return self.fc2(MF.gelu(self.fc1(h), *self.drop_args()))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.fused:
+            y = self.mlp(MF.layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps))
+            rate, seed = self.drop_args()
+            if not self.residual and rate == 0.0:
+                return y
+            return MF.dropout(y, rate, seed, residual=x if self.residual else None)
         y = self.fc2(self.act(self.fc1(self.norm(x))))
         return x + y if self.residual else y
 
     def vcon_step(self) -> None:
         self.fc1.vcon_step()
         self.fc2.vcon_step()
+
+
+class MAMMlpStack(nn.Module):
+    """`depth` fused MLP blocks and the final norm of the encoder (`vit.layernorm` of a Hugging Face ViT):
+    LayerNorm(block_depth(... block_1(x))).  The residual stream and the next norm's output come out of one pass."""
+
+    def __init__(self, depth: int, hidden: int = 768, intermediate: int = 3072, layer_norm_eps: float = 1e-12,
+                 drop_rate: float = 0.0, device=None, dtype=None, **block_kwargs):
+        super().__init__()
+        if depth < 1:
+            raise ValueError("depth must be at least 1")
+        self.blocks = nn.ModuleList(
+            MAMMlpBlock(hidden, intermediate, layer_norm_eps=layer_norm_eps, device=device, dtype=dtype, fused=True,
+                        drop_rate=drop_rate, **block_kwargs) for _ in range(depth))
+        if not self.blocks[0].residual:
+            raise ValueError("the blocks of a stack have residuals")
+        self.norm = nn.LayerNorm(hidden, eps=layer_norm_eps, device=device, dtype=dtype)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        norms = [block.norm for block in self.blocks] + [self.norm]
+        h = MF.layer_norm(x, norms[0].weight, norms[0].bias, norms[0].eps)
+        for block, norm in zip(self.blocks, norms[1:]):
+            h, x = MF.dropout_add_layer_norm(block.mlp(h), x, norm.weight, norm.bias, norm.eps, *block.drop_args())
+        return h
+
+    def vcon_step(self) -> None:
+        for block in self.blocks:
+            block.vcon_step()
 
 
 class GraphedStep:
