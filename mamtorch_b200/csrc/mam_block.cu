@@ -1,5 +1,6 @@
 // C ABI of the operators between the MAM layers of a transformer block: layer norm, dropout with residual addition, GELU.
 // Declarations are in include/mam_b200.h.
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -150,6 +151,27 @@ BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, 
     return b;
 }
 
+// Lets a kernel have `bytes` of dynamic shared memory; asked of the runtime once for each device and size that is larger.
+template <auto KERNEL>
+int allow_smem(int bytes) {
+    static std::atomic<int> allowed[64];
+    int dev = 0;
+    MAM_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
+    if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return MAM_OK;
+    MAM_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    allowed[dev].store(bytes, std::memory_order_relaxed);
+    return MAM_OK;
+}
+
+template <typename T, int NV, bool ADD, int MODE>
+int ring_run(const NormBwdParams& p, const BwdPlan& b, const BwdRing& r, cudaStream_t st) {
+    const int e = allow_smem<mam_norm_bwd_ring_kernel<T, NV, ADD, MODE>>((int)r.bytes);
+    if (e != MAM_OK) return e;
+    mam_norm_bwd_ring_kernel<T, NV, ADD, MODE><<<(unsigned)b.parts, b.group * b.groups, r.bytes, st>>>(p, r);
+    MAM_CUDA(cudaGetLastError());
+    return MAM_OK;
+}
 template <typename T, int NV, bool ADD>
 int ring_launch(const NormBwdParams& p, const BwdPlan& b, const DevInfo& d, cudaStream_t st) {
     BwdRing r{};
@@ -162,33 +184,30 @@ int ring_launch(const NormBwdParams& p, const BwdPlan& b, const DevInfo& d, cuda
     r.weights_at = (unsigned)((row * r.stages + 127) / 128 * 128);
     r.bars_at = (unsigned)(r.weights_at + (p.width * 4 + 15) / 16 * 16);
     r.bytes = r.bars_at + b.groups * r.stages * 8;
-    const auto run = [&](auto kernel) -> int {
-        MAM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)r.bytes));
-        kernel<<<(unsigned)b.parts, b.group * b.groups, r.bytes, st>>>(p, r);
-        MAM_CUDA(cudaGetLastError());
-        return MAM_OK;
-    };
-    if (p.width == (long long)b.group * NV * VEC<T>) return run(mam_norm_bwd_ring_kernel<T, NV, ADD, FULL>);
-    return run(mam_norm_bwd_ring_kernel<T, NV, ADD, ALIGNED>);
+    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<T, NV, ADD, FULL>(p, b, r, st);
+    return ring_run<T, NV, ADD, ALIGNED>(p, b, r, st);
 }
 
-template <typename T, int NV, bool ADD, int MODE>
-int bwd_launch(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
+template <typename T, int NV, bool ADD, int MODE, int LANES>
+int bwd_run(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
     const int rows = b.group < 32 ? b.group * b.groups / 32 : b.groups;
     const size_t smem = rows > 1 ? (size_t)rows * 2 * (size_t)p.width * 4 : 0;
-    const auto run = [&](auto kernel) -> int {
-        if (smem > 40 * 1024)
-            MAM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        kernel<<<(unsigned)b.parts, b.group * b.groups, smem, st>>>(p, b.group);
-        MAM_CUDA(cudaGetLastError());
-        return MAM_OK;
-    };
+    if (smem > 40 * 1024) {
+        const int e = allow_smem<mam_norm_bwd_kernel<T, NV, ADD, MODE, LANES>>((int)smem);
+        if (e != MAM_OK) return e;
+    }
+    mam_norm_bwd_kernel<T, NV, ADD, MODE, LANES><<<(unsigned)b.parts, b.group * b.groups, smem, st>>>(p, b.group);
+    MAM_CUDA(cudaGetLastError());
+    return MAM_OK;
+}
+template <typename T, int NV, bool ADD, int MODE>
+int bwd_launch(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
     if constexpr (MODE == RAGGED) {
-        if (b.group >= 32) return run(mam_norm_bwd_kernel<T, NV, ADD, MODE, 32>);
+        if (b.group >= 32) return bwd_run<T, NV, ADD, MODE, 32>(p, b, st);
     }
     if constexpr (NV * VEC<T> == 8) {
-        if (b.group == 8) return run(mam_norm_bwd_kernel<T, NV, ADD, MODE, 8>);
-        return run(mam_norm_bwd_kernel<T, NV, ADD, MODE, 16>);
+        if (b.group == 8) return bwd_run<T, NV, ADD, MODE, 8>(p, b, st);
+        return bwd_run<T, NV, ADD, MODE, 16>(p, b, st);
     }
     return MAM_ERR_UNSUPPORTED;
 }

@@ -2,14 +2,17 @@
 //
 // The `*_forward` / `*_backward` operators validate, allocate and call the library (CUDA only: a CPU tensor gets the
 // dispatcher's NotImplementedError).  The differentiable ones (layer_norm, dropout_add_layer_norm, dropout, gelu) call
-// them below a C++ autograd node where a gradient is wanted, and directly where none is: for a few rows the host's time
+// them below an autograd node where a gradient is wanted, and directly where none is: for a few rows the host's time
 // is the call's time.
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <vector>
@@ -20,7 +23,7 @@ namespace {
 
 using at::Tensor;
 using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 void check_status(int st, const char* what) {
@@ -92,6 +95,12 @@ Tensor as_rows(const Tensor& t, int64_t& pitch) {
     return t.contiguous();
 }
 
+// a contiguous tensor without the dispatcher's detour: for a few rows these calls are a tenth of the operator's time
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType t, const Tensor& like) {
+    return at::detail::empty_cuda(sizes, t, like.device(), std::nullopt);
+}
+Tensor fresh(const Tensor& like) { return fresh(like.sizes(), like.scalar_type(), like); }
+
 // ---------------------------------------------------------------- CUDA operators
 
 std::vector<Tensor> layer_norm_forward(const Tensor& x, const OptTensor& residual, const OptTensor& weight,
@@ -110,9 +119,11 @@ std::vector<Tensor> layer_norm_forward(const Tensor& x, const OptTensor& residua
     int64_t xp = 0, rp = 0;
     const Tensor xr = as_rows(x, xp), rr = has(residual) ? as_rows(*residual, rp) : Tensor();
     const int64_t width = x.size(-1), rows = x.numel() / width;
-    std::vector<Tensor> out{at::empty(x.sizes(), x.options())};
-    if (rr.defined()) out.push_back(at::empty(x.sizes(), x.options()));
-    if (want_stats) out.push_back(at::empty({rows, 2}, x.options().dtype(at::kFloat)));
+    std::vector<Tensor> out;
+    out.reserve(3);
+    out.push_back(fresh(x));
+    if (rr.defined()) out.push_back(fresh(x));
+    if (want_stats) out.push_back(fresh({rows, 2}, at::kFloat, x));
     if (rows == 0) return out;
     check_status(mam_layer_norm_fwd(ptr(xr), xp, ptr(rr), rp, ptr(w), ptr(b), pdtype, (float)eps, (float)rate,
                                     (uint64_t)seed, seed_ptr(seed_at), mut(out[0]), rr.defined() ? mut(out[1]) : nullptr,
@@ -122,7 +133,7 @@ std::vector<Tensor> layer_norm_forward(const Tensor& x, const OptTensor& residua
     return out;
 }
 
-// ds, dx (where something is dropped; else ds is the gradient of x too), dweight, dbias; those not wanted are empty
+// ds, dx (where something is dropped; else ds is the gradient of x too), dweight, dbias: those that are wanted
 std::vector<Tensor> layer_norm_backward(const OptTensor& gy, const OptTensor& gsum, const Tensor& s, const Tensor& stats,
                                         const OptTensor& weight, double rate, int64_t seed, const OptTensor& seed_at,
                                         bool params_f32, bool want_weight, bool want_bias) {
@@ -143,23 +154,28 @@ std::vector<Tensor> layer_norm_backward(const OptTensor& gy, const OptTensor& gs
     const Tensor g = has(gy) ? gy->contiguous() : Tensor(), gs = has(gsum) ? gsum->contiguous() : Tensor();
     int64_t sp = 0;
     const Tensor sr = as_rows(s, sp);
-    Tensor ds = at::empty(s.sizes(), s.options()), dx, dw, db;
-    if (rate > 0) dx = at::empty(s.sizes(), s.options());
-    const auto popt = s.options().dtype(pdtype == MAM_F32 ? at::kFloat : s.scalar_type());
-    if (want_weight) dw = rows ? at::empty({width}, popt) : at::zeros({width}, popt);
-    if (want_bias) db = rows ? at::empty({width}, popt) : at::zeros({width}, popt);
+    Tensor ds = fresh(s), dx, dw, db;
+    if (rate > 0) dx = fresh(s);
+    const at::ScalarType kind = pdtype == MAM_F32 ? at::kFloat : s.scalar_type();
+    if (want_weight) dw = fresh({width}, kind, s);
+    if (want_bias) db = fresh({width}, kind, s);
     if (rows) {
         const size_t bytes = want_weight || want_bias ? mam_layer_norm_bwd_workspace_bytes(rows, width) : 0;
         Tensor ws;
-        if (bytes) ws = at::empty({(int64_t)bytes}, s.options().dtype(at::kByte));
+        if (bytes) ws = fresh({(int64_t)bytes}, at::kByte, s);
         check_status(mam_layer_norm_bwd(ptr(g), ptr(gs), ptr(sr), sp, stats.const_data_ptr<float>(), ptr(w), pdtype,
                                         (float)rate, (uint64_t)seed, seed_ptr(seed_at), mut(ds), mut(dx), mut(dw),
                                         mut(db), rows, width, dtype, mut(ws), bytes,
                                         at::cuda::getCurrentCUDAStream().stream()),
                      "mam_layer_norm_bwd");
     }
-    const auto none = [&] { return at::empty({0}, s.options()); };
-    return {ds, dx.defined() ? dx : none(), dw.defined() ? dw : none(), db.defined() ? db : none()};
+    std::vector<Tensor> out;
+    out.reserve(4);
+    for (Tensor* g : {&ds, &dx, &dw, &db})
+        if (g->defined()) out.push_back(std::move(*g));
+    if (rows == 0)
+        for (auto& g : out) g.zero_();
+    return out;
 }
 
 Tensor dropout_forward(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
@@ -169,7 +185,7 @@ Tensor dropout_forward(const Tensor& x, const OptTensor& residual, double rate, 
     if (has(residual)) check_like(*residual, x, "residual");
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor xc = x.contiguous(), rc = has(residual) ? residual->contiguous() : Tensor();
-    Tensor y = at::empty(x.sizes(), x.options());
+    Tensor y = fresh(x);
     if (y.numel())
         check_status(mam_dropout_add(ptr(xc), ptr(rc), mut(y), y.numel(), dtype, (float)rate, (uint64_t)seed,
                                      seed_ptr(seed_at), at::cuda::getCurrentCUDAStream().stream()),
@@ -183,7 +199,7 @@ Tensor gelu_forward(const Tensor& x, double rate, int64_t seed, const OptTensor&
     check_drop(x, rate, seed_at);
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor xc = x.contiguous();
-    Tensor y = at::empty(x.sizes(), x.options());
+    Tensor y = fresh(x);
     if (y.numel())
         check_status(mam_gelu_fwd(ptr(xc), mut(y), y.numel(), dtype, (float)rate, (uint64_t)seed, seed_ptr(seed_at),
                                   at::cuda::getCurrentCUDAStream().stream()),
@@ -198,7 +214,7 @@ Tensor gelu_backward(const Tensor& gy, const Tensor& x, double rate, int64_t see
     check_like(gy, x, "the gradient of y");
     c10::cuda::CUDAGuard guard(x.device());
     const Tensor gc = gy.contiguous(), xc = x.contiguous();
-    Tensor dx = at::empty(x.sizes(), x.options());
+    Tensor dx = fresh(x);
     if (dx.numel())
         check_status(mam_gelu_bwd(ptr(gc), ptr(xc), mut(dx), dx.numel(), dtype, (float)rate, (uint64_t)seed,
                                   seed_ptr(seed_at), at::cuda::getCurrentCUDAStream().stream()),
@@ -220,135 +236,160 @@ bool wants_grad(const Ts&... ts) {
 Tensor plain(const OptTensor& t) { return has(t) ? *t : Tensor(); }
 
 // Gradients are not differentiable again: under create_graph they carry a node that says so when it is run.
-void once(variable_list& grads, bool graph) {
-    if (!graph) return;
-    for (auto& g : grads)
-        if (g.defined())
-            g = (*std::make_shared<torch::autograd::DelayedError>(
-                "mamtorch_b200: layer_norm, dropout and gelu are differentiable once", 1))(
-                {g.detach().requires_grad_(true)})[0];
+variable_list once(variable_list&& grads, bool graph) {
+    if (graph)
+        for (auto& g : grads)
+            if (g.defined())
+                g = (*std::make_shared<torch::autograd::DelayedError>(
+                    "mamtorch_b200: layer_norm, dropout and gelu are differentiable once", 1))(
+                    {g.detach().requires_grad_(true)})[0];
+    return std::move(grads);
 }
 
-struct NormFn : torch::autograd::Function<NormFn> {
-    static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual,
-                                 const OptTensor& weight, const OptTensor& bias, const OptTensor& seed_at, double eps,
-                                 double rate, int64_t seed) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        MAM_OP(op, layer_norm_forward);
-        auto out = op.call(x, residual, weight, bias, eps, rate, seed, seed_at, true);
-        ctx->set_materialize_grads(false);
-        ctx->save_for_backward({has(residual) ? out[1] : x, out.back(), plain(weight), plain(seed_at)});
-        ctx->saved_data["rate"] = rate;
-        ctx->saved_data["seed"] = seed;
-        const Tensor param = has(weight) ? *weight : plain(bias);
-        ctx->saved_data["f32"] = param.defined() && param.scalar_type() == at::kFloat;
-        ctx->saved_data["given"] = (int64_t)(has(residual) | has(weight) << 1 | has(bias) << 2);
-        out.pop_back();
-        return out;
+// The nodes are written out, as torch's own are: the generic C++ Function keeps its arguments in a dictionary by name, which
+// took as long as an allocation.
+struct BlockNode : torch::autograd::Node {
+    double rate = 0;
+    int64_t seed = 0;
+    SavedVariable seed_at;
+    void release_variables() override { seed_at.reset_data(); }
+};
+template <class N, class... Ts>
+std::shared_ptr<N> make_node(double rate, int64_t seed, const OptTensor& seed_at, const Ts&... inputs) {
+    std::shared_ptr<N> n(new N(), torch::autograd::deleteNode);
+    n->rate = rate;
+    n->seed = seed;
+    if (has(seed_at)) n->seed_at = SavedVariable(*seed_at, false);
+    n->set_next_edges(torch::autograd::collect_next_edges(inputs...));
+    return n;
+}
+
+struct NormBackward : BlockNode {       // inputs: x, residual, weight, bias
+    SavedVariable s, stats, weight;
+    bool add = false, f32 = false;
+    std::string name() const override { return "MamLayerNormBackward"; }
+    void release_variables() override {
+        BlockNode::release_variables();
+        s.reset_data();
+        stats.reset_data();
+        weight.reset_data();
     }
-    static variable_list backward(AutogradContext* ctx, variable_list g) {
+    variable_list apply(variable_list&& g) override {
         const bool graph = at::GradMode::is_enabled();
         at::AutoGradMode off(false);
-        const auto saved = ctx->get_saved_variables();
-        const int64_t given = ctx->saved_data["given"].toInt();
-        const bool add = given & 1;
-        // the node has an edge for each tensor that was given, in the order of the arguments
-        size_t edge = 0;
-        const auto wanted = [&](bool there) { return there && ctx->needs_input_grad(edge++); };
-        const bool want_x = wanted(true), want_res = wanted(add), want_w = wanted(given & 2), want_b = wanted(given & 4);
-        const double rate = ctx->saved_data["rate"].toDouble();
         const Tensor gs = add ? g[1] : Tensor();
-        variable_list r(8);
-        if (!g[0].defined() && !gs.defined()) return r;
-        MAM_OP(op, layer_norm_backward);
-        auto d = op.call(opt(g[0]), opt(gs), saved[0], saved[1], opt(saved[2]), rate, ctx->saved_data["seed"].toInt(),
-                         opt(saved[3]), ctx->saved_data["f32"].toBool(), want_w, want_b);
-        if (want_x) r[0] = rate > 0 ? d[1] : d[0];
-        if (want_res) r[1] = d[0];
-        if (want_w) r[2] = d[2];
-        if (want_b) r[3] = d[3];
-        once(r, graph);
-        return r;
-    }
-};
-
-struct DropoutFn : torch::autograd::Function<DropoutFn> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const OptTensor& seed_at,
-                          double rate, int64_t seed) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        MAM_OP(op, dropout_forward);
-        ctx->save_for_backward({plain(seed_at)});
-        ctx->saved_data["add"] = has(residual);
-        ctx->saved_data["rate"] = rate;
-        ctx->saved_data["seed"] = seed;
-        return op.call(x, residual, rate, seed, seed_at);
-    }
-    static variable_list backward(AutogradContext* ctx, variable_list g) {
-        const bool graph = at::GradMode::is_enabled();
-        at::AutoGradMode off(false);
-        const double rate = ctx->saved_data["rate"].toDouble();
-        variable_list r(5);
-        if (!g[0].defined()) return r;
-        if (ctx->needs_input_grad(0)) {
-            MAM_OP(op, dropout_forward);
-            r[0] = rate > 0 ? op.call(g[0], std::nullopt, rate, ctx->saved_data["seed"].toInt(),
-                                      opt(ctx->get_saved_variables()[0]))
-                            : g[0];
-        }
-        if (ctx->saved_data["add"].toBool() && ctx->needs_input_grad(1)) r[1] = g[0];
-        once(r, graph);
-        return r;
-    }
-};
-
-struct GeluFn : torch::autograd::Function<GeluFn> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& seed_at, double rate, int64_t seed) {
-        at::AutoDispatchBelowADInplaceOrView below;
-        MAM_OP(op, gelu_forward);
-        ctx->save_for_backward({x, plain(seed_at)});
-        ctx->saved_data["rate"] = rate;
-        ctx->saved_data["seed"] = seed;
-        return op.call(x, rate, seed, seed_at);
-    }
-    static variable_list backward(AutogradContext* ctx, variable_list g) {
-        const bool graph = at::GradMode::is_enabled();
-        at::AutoGradMode off(false);
         variable_list r(4);
-        if (!g[0].defined() || !ctx->needs_input_grad(0)) return r;
-        const auto saved = ctx->get_saved_variables();
-        MAM_OP(op, gelu_backward);
-        r[0] = op.call(g[0], saved[0], ctx->saved_data["rate"].toDouble(), ctx->saved_data["seed"].toInt(), opt(saved[1]));
-        once(r, graph);
-        return r;
+        if (!g[0].defined() && !gs.defined()) return r;
+        const auto self = shared_from_this();
+        const Tensor w = weight.unpack(), at = seed_at.unpack();
+        const bool want_w = task_should_compute_output(2), want_b = task_should_compute_output(3);
+        MAM_OP(op, layer_norm_backward);
+        auto d = op.call(opt(g[0]), opt(gs), s.unpack(add ? self : nullptr), stats.unpack(), opt(w), rate, seed, opt(at), f32,
+                         want_w, want_b);
+        size_t next = 1;
+        if (task_should_compute_output(1)) r[1] = d[0];
+        if (rate > 0) {
+            if (task_should_compute_output(0)) r[0] = std::move(d[next]);
+            ++next;
+        } else if (task_should_compute_output(0)) {
+            r[0] = d[0];
+        }
+        if (want_w) r[2] = std::move(d[next++]);
+        if (want_b) r[3] = std::move(d[next]);
+        return once(std::move(r), graph);
     }
 };
 
-Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
-    if (wants_grad(x, plain(weight), plain(bias)))
-        return NormFn::apply(x, std::nullopt, weight, bias, std::nullopt, eps, 0.0, 0)[0];
+struct DropoutBackward : BlockNode {    // inputs: x, residual
+    std::string name() const override { return "MamDropoutBackward"; }
+    variable_list apply(variable_list&& g) override {
+        const bool graph = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        variable_list r(2);
+        if (!g[0].defined()) return r;
+        if (task_should_compute_output(0)) {
+            MAM_OP(op, dropout_forward);
+            r[0] = rate > 0 ? op.call(g[0], std::nullopt, rate, seed, opt(seed_at.unpack())) : g[0];
+        }
+        if (task_should_compute_output(1)) r[1] = g[0];
+        return once(std::move(r), graph);
+    }
+};
+
+struct GeluBackward : BlockNode {       // input: x
+    SavedVariable x;
+    std::string name() const override { return "MamGeluBackward"; }
+    void release_variables() override {
+        BlockNode::release_variables();
+        x.reset_data();
+    }
+    variable_list apply(variable_list&& g) override {
+        const bool graph = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        variable_list r(1);
+        if (!g[0].defined()) return r;
+        MAM_OP(op, gelu_backward);
+        r[0] = op.call(g[0], x.unpack(), rate, seed, opt(seed_at.unpack()));
+        return once(std::move(r), graph);
+    }
+};
+
+// y, s with a residual
+std::vector<Tensor> norm(const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias,
+                         double eps, double rate, int64_t seed, const OptTensor& seed_at) {
     MAM_OP(op, layer_norm_forward);
-    return op.call(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt, false)[0];
+    const Tensor res = plain(residual), w = plain(weight), b = plain(bias);
+    if (!wants_grad(x, res, w, b)) return op.call(x, residual, weight, bias, eps, rate, seed, seed_at, false);
+    auto node = make_node<NormBackward>(rate, seed, seed_at, x, res, w, b);
+    std::vector<Tensor> out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        out = op.call(x, residual, weight, bias, eps, rate, seed, seed_at, true);
+    }
+    node->stats = SavedVariable(out.back(), false);
+    out.pop_back();
+    node->add = res.defined();
+    const Tensor& param = w.defined() ? w : b;
+    node->f32 = param.defined() && param.scalar_type() == at::kFloat;
+    node->weight = SavedVariable(w, false);
+    for (auto& y : out) torch::autograd::set_history(y, node);
+    node->s = res.defined() ? SavedVariable(out[1], true) : SavedVariable(x, false);
+    return out;
+}
+Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    return norm(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt)[0];
 }
 std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
                                                   const OptTensor& bias, double eps, double rate, int64_t seed,
                                                   const OptTensor& seed_at) {
-    if (wants_grad(x, residual, plain(weight), plain(bias))) {
-        auto out = NormFn::apply(x, residual, weight, bias, seed_at, eps, rate, seed);
-        return {out[0], out[1]};
-    }
-    MAM_OP(op, layer_norm_forward);
-    auto out = op.call(x, residual, weight, bias, eps, rate, seed, seed_at, false);
-    return {out[0], out[1]};
+    auto out = norm(x, residual, weight, bias, eps, rate, seed, seed_at);
+    return {std::move(out[0]), std::move(out[1])};
 }
 Tensor dropout(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
-    if (wants_grad(x, plain(residual))) return DropoutFn::apply(x, residual, seed_at, rate, seed);
     MAM_OP(op, dropout_forward);
-    return op.call(x, residual, rate, seed, seed_at);
+    const Tensor res = plain(residual);
+    if (!wants_grad(x, res)) return op.call(x, residual, rate, seed, seed_at);
+    auto node = make_node<DropoutBackward>(rate, seed, seed_at, x, res);
+    Tensor y;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = op.call(x, residual, rate, seed, seed_at);
+    }
+    torch::autograd::set_history(y, node);
+    return y;
 }
 Tensor gelu(const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
-    if (wants_grad(x)) return GeluFn::apply(x, seed_at, rate, seed);
     MAM_OP(op, gelu_forward);
-    return op.call(x, rate, seed, seed_at);
+    if (!wants_grad(x)) return op.call(x, rate, seed, seed_at);
+    auto node = make_node<GeluBackward>(rate, seed, seed_at, x);
+    Tensor y;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        y = op.call(x, rate, seed, seed_at);
+    }
+    node->x = SavedVariable(x, false);
+    torch::autograd::set_history(y, node);
+    return y;
 }
 
 }  // namespace

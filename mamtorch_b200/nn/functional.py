@@ -173,10 +173,8 @@ def _(x, residual, weight, bias, eps, drop_rate, drop_seed, drop_seed_at, want_s
 @torch.library.register_fake("mamtorch_b200::layer_norm_backward")
 def _(gy, gsum, s, stats, weight, drop_rate, drop_seed, drop_seed_at, params_f32, want_weight, want_bias):
     kind = torch.float if params_f32 else s.dtype
-    none = s.new_empty((0,))
-    return [s.new_empty(s.shape), s.new_empty(s.shape) if drop_rate > 0 else none,
-            s.new_empty((s.size(-1),), dtype=kind) if want_weight else none,
-            s.new_empty((s.size(-1),), dtype=kind) if want_bias else none]
+    return ([s.new_empty(s.shape) for _ in range(2 if drop_rate > 0 else 1)]
+            + [s.new_empty((s.size(-1),), dtype=kind) for _ in range(int(want_weight) + int(want_bias))])
 
 
 @torch.library.register_fake("mamtorch_b200::dropout_forward")
