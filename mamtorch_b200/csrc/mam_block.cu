@@ -100,9 +100,9 @@ int ring_stages(int64_t width, int groups, int size, int tensors, const DevInfo&
 // Most partial rows of a backward: a CTA an SM, or the slabs of the wide form.
 long long bwd_parts(int64_t rows, int64_t width, int sms) {
     if (width <= 8192) return rows < sms ? rows : sms;
-    const long long groups = (width + NORM_COLS - 1) / NORM_COLS;
-    const long long slabs = (8LL * sms + groups - 1) / groups, most = (rows + 63) / 64;
-    return slabs < most ? slabs : most;
+    const long long groups = (width + 127) / 128;      // a CTA's columns in fp32; 16-bit types have half as many CTAs
+    const long long slabs = 8LL * sms / groups, most = (rows + 31) / 32;
+    return slabs < 1 ? 1 : slabs < most ? slabs : most;
 }
 
 BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, const DevInfo& d) {
@@ -220,6 +220,15 @@ int bwd_mode(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevIn
     return MAM_ERR_UNSUPPORTED;
 }
 
+template <typename T, bool ADD, int MODE>
+void wide_launch(const NormBwdParams& p, cudaStream_t st) {
+    const unsigned rows = (unsigned)p.rows;
+    // CTAs of half the size where they suffice: two rows at a time on an SM
+    if (p.width <= 4096 * VEC<T>)
+        mam_norm_bwd_wide_kernel<T, 4, ADD, MODE><<<rows, p.width <= 2048 * VEC<T> ? 512 : 1024, 0, st>>>(p);
+    else mam_norm_bwd_wide_kernel<T, 0, ADD, MODE><<<rows, 1024, 0, st>>>(p);
+}
+
 template <typename T, bool ADD>
 int bwd_pick(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
     if (b.kind != BwdPlan::WIDE) {
@@ -227,12 +236,13 @@ int bwd_pick(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevIn
         if (b.per == 16) return bwd_mode<T, 16 / VEC<T>, ADD>(p, b, aligned, d, st);
         return bwd_mode<T, 24 / VEC<T>, ADD>(p, b, aligned, d, st);
     }
-    if (aligned) mam_norm_bwd_wide_kernel<T, ADD, ALIGNED><<<(unsigned)p.rows, 1024, 0, st>>>(p);
-    else mam_norm_bwd_wide_kernel<T, ADD, RAGGED><<<(unsigned)p.rows, 1024, 0, st>>>(p);
+    if (aligned) wide_launch<T, ADD, ALIGNED>(p, st);
+    else wide_launch<T, ADD, RAGGED>(p, st);
     if (p.partial) {
         const long long per = (p.rows + b.parts - 1) / b.parts;
-        mam_norm_bwd_cols_kernel<T><<<dim3((unsigned)((p.width + NORM_COLS - 1) / NORM_COLS), (unsigned)b.parts),
-                                      NORM_COLS * NORM_LANES, 0, st>>>(p, per);
+        const dim3 grid((unsigned)((p.width + NORM_COLS * VEC<T> - 1) / (NORM_COLS * VEC<T>)), (unsigned)b.parts);
+        if (aligned) mam_norm_bwd_cols_kernel<T, ALIGNED><<<grid, NORM_COLS * NORM_LANES, 0, st>>>(p, per);
+        else mam_norm_bwd_cols_kernel<T, RAGGED><<<grid, NORM_COLS * NORM_LANES, 0, st>>>(p, per);
     }
     MAM_CUDA(cudaGetLastError());
     return MAM_OK;

@@ -631,30 +631,32 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
     }
 }
 
-// Backward of rows of any width: gradients of the rows, one CTA a row, without the columns' sums.
-template <typename T, bool ADD, int MODE>
+// Backward of rows of any width: gradients of the rows, one CTA a row, without the columns' sums.  NV > 0: the row's vectors,
+// NV a thread, stay in registers as they were read; 0: they are read again.
+template <typename T, int NV, bool ADD, int MODE>
 __global__ void __launch_bounds__(1024) mam_norm_bwd_wide_kernel(const __grid_constant__ NormBwdParams p) {
     __shared__ float2 slot[32];
-    constexpr int V = VEC<T>;
+    constexpr int V = VEC<T>, KEPT = NV > 0 ? NV : 1;
     const long long row = blockIdx.x, width = p.width, step = (long long)blockDim.x * V;
     const long long first = (long long)(threadIdx.x & ~31) * V;
     const int lane = threadIdx.x & 31;
     const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy), *gs0 = static_cast<const T*>(p.gs);
     const RowSrc<T, MODE> s(s0, p.s_pitch, p.rows, width, s0 + row * p.s_pitch),
         gy(gy0, width, p.rows, width, gy0 + row * width), gs(gs0, width, p.rows, width, gs0 + row * width);
-    uint4 none;
+    uint4 none, qs[KEPT], qg[KEPT];
     const float2 st = p.stats[row];
     const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
     const unsigned long long seed = ADD && p.drop.on ? p.drop.seed_now() : 0;
     auto count = [&](long long c) { return (int)min((long long)V, width - c); };
+    auto get = [&](long long c, int i) {
+        qs[i] = s.load(c, count(c));
+        qg[i] = p.gy ? gy.load(c, count(c)) : make_uint4(0u, 0u, 0u, 0u);
+    };
     // normalised values and weighted gradients of the vector at c
-    auto get = [&](long long c, Vals<T>& h, Vals<T>& a) {
+    auto values = [&](long long c, int i, Vals<T>& h, Vals<T>& a) {
         Vals<T> w;
-        unpack<T>(s.load(c, count(c)), h);
-        if (p.gy) unpack<T>(gy.load(c, count(c)), a);
-        else
-#pragma unroll
-            for (int j = 0; j < V / 2; ++j) a[j] = splat2(0.f);
+        unpack<T>(qs[i], h);
+        unpack<T>(qg[i], a);
         load_param<T, MODE>(p.weight, p.params_f32, (int)c, count(c), 1.f, w);
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) {
@@ -667,23 +669,35 @@ __global__ void __launch_bounds__(1024) mam_norm_bwd_wide_kernel(const __grid_co
         }
     };
     float2 s1 = splat2(0.f), s2 = s1;
-    if (p.gy)
-        for (long long c = first + lane * V; c < width; c += step) {
-            Vals<T> h, a;
-            get(c, h, a);
-            s1 = add2(s1, total<T>(a));
+    auto add = [&](long long c, int i) {
+        Vals<T> h, a;
+        values(c, i, h, a);
+        s1 = add2(s1, total<T>(a));
 #pragma unroll
-            for (int j = 0; j < V / 2; ++j) s2 = fma2(a[j], h[j], s2);
+        for (int j = 0; j < V / 2; ++j) s2 = fma2(a[j], h[j], s2);
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (first + lane * V + i * step < width) get(first + lane * V + i * step, i);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (first + lane * V + i * step < width) add(first + lane * V + i * step, i);
+    } else if (p.gy) {
+        for (long long c = first + lane * V; c < width; c += step) {
+            get(c, 0);
+            add(c, 0);
         }
+    }
     const float2 m = row_sum2<true, 32, 32>(sum2(s1), sum2(s2), slot);
     const float2 c1 = splat2(-st.y * (m.x * p.inv_width)), c2 = splat2(-st.y * (m.y * p.inv_width));
-    for (long long c0 = first; c0 < width; c0 += step) {
-        const long long c = c0 + lane * V, at = row * width + c;
+    auto finish = [&](long long c, int i) {
+        const long long at = row * width + c;
         const int rest = (int)min(width - c, (long long)2 * V);
         uint4 q = make_uint4(0u, 0u, 0u, 0u), qd = q;
         if (rest > 0) {
             Vals<T> h, a;
-            get(c, h, a);
+            values(c, i, h, a);
 #pragma unroll
             for (int j = 0; j < V / 2; ++j) a[j] = fma2(a[j], r2, fma2(h[j], c2, c1));
             if constexpr (ADD) {
@@ -706,38 +720,70 @@ __global__ void __launch_bounds__(1024) mam_norm_bwd_wide_kernel(const __grid_co
         if constexpr (ADD) {
             if (p.dx) store_vec<T, MODE>(static_cast<T*>(p.dx) + at, qd, rest, lane, 32, true, true, none);
         }
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (first + i * step < width) finish(first + lane * V + i * step, i);
+    } else {
+        for (long long c0 = first; c0 < width; c0 += step) {
+            const long long c = c0 + lane * V;
+            if (c < width) get(c, 0);
+            finish(c, 0);
+        }
     }
 }
 
 constexpr int NORM_COLS = 32, NORM_LANES = 8;
 
-// The columns' sums of gy h and gy over slabs of rows, for rows wider than a CTA's registers hold: grid (column groups,
-// slabs), into partial[slab][2][width].
-template <typename T>
-__global__ void __launch_bounds__(NORM_COLS * NORM_LANES)
+// The columns' sums of gy h and gy over slabs of rows, for rows wider than a CTA's registers hold: grid (groups of 32
+// vectors, slabs), into partial[slab][2][width].  Column by column it read 64 bytes of a row at a time and took longer than
+// the rows' own kernel.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(NORM_COLS * NORM_LANES, 4)
 mam_norm_bwd_cols_kernel(const __grid_constant__ NormBwdParams p, long long rows_per) {
-    __shared__ float2 part[NORM_LANES][NORM_COLS];
-    const int c = threadIdx.x % NORM_COLS, l = threadIdx.x / NORM_COLS;
-    const long long n = (long long)blockIdx.x * NORM_COLS + c;
+    constexpr int V = VEC<T>;
+    __shared__ float part[NORM_LANES][2][NORM_COLS * V];
+    const int lane = threadIdx.x % NORM_COLS, l = threadIdx.x / NORM_COLS;
+    const long long c = ((long long)blockIdx.x * NORM_COLS + lane) * V;
     const long long m0 = (long long)blockIdx.y * rows_per, m1 = min(m0 + rows_per, p.rows);
-    float2 sum = make_float2(0.f, 0.f);
-    if (n < p.width && p.gy)
+    const int n = (int)min((long long)V, p.width - c);
+    const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy);
+    float2 aw[V / 2], ab[V / 2];
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) aw[j] = ab[j] = splat2(0.f);
+    if (n > 0 && gy0)
+#pragma unroll 4
         for (long long m = m0 + l; m < m1; m += NORM_LANES) {
+            const RowSrc<T, MODE> s(s0, p.s_pitch, p.rows, p.width, s0 + m * p.s_pitch),
+                gy(gy0, p.width, p.rows, p.width, gy0 + m * p.width);
+            const uint4 qs = s.load(c, n), qg = gy.load(c, n);
             const float2 st = p.stats[m];
-            const float a = to_f32(static_cast<const T*>(p.gy)[m * p.width + n]);
-            sum.x = fmaf(a, (to_f32(static_cast<const T*>(p.s)[m * p.s_pitch + n]) - st.x) * st.y, sum.x);
-            sum.y += a;
+            Vals<T> h, a;
+            unpack<T>(qs, h);
+            unpack<T>(qg, a);
+            const float2 minus = splat2(-st.x), r2 = splat2(st.y);
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {
+                aw[j] = fma2(a[j], mul2(add2(h[j], minus), r2), aw[j]);
+                ab[j] = add2(ab[j], a[j]);
+            }
         }
-    part[l][c] = sum;
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) {
+        *reinterpret_cast<float2*>(&part[l][0][lane * V + 2 * j]) = aw[j];
+        *reinterpret_cast<float2*>(&part[l][1][lane * V + 2 * j]) = ab[j];
+    }
     __syncthreads();
-    if (l == 0 && n < p.width) {
-        for (int i = 1; i < NORM_LANES; ++i) {
-            sum.x += part[i][c].x;
-            sum.y += part[i][c].y;
-        }
-        float* out = p.partial + (long long)blockIdx.y * 2 * p.width;
-        out[n] = sum.x;
-        out[p.width + n] = sum.y;
+    float* out = p.partial + (long long)blockIdx.y * 2 * p.width;
+    for (int k = threadIdx.x; k < 2 * NORM_COLS * V; k += NORM_COLS * NORM_LANES) {
+        const int which = k / (NORM_COLS * V), at = k % (NORM_COLS * V);
+        const long long to = (long long)blockIdx.x * NORM_COLS * V + at;
+        if (to >= p.width) continue;      // what lies behind a row's end is not a number to be had
+        float sum = part[0][which][at];
+#pragma unroll
+        for (int i = 1; i < NORM_LANES; ++i) sum += part[i][which][at];
+        out[which * p.width + to] = sum;
     }
 }
 
