@@ -83,16 +83,20 @@ void fwd_pick(const NormFwdParams& p, bool aligned, const DevInfo& d, cudaStream
 
 // ---- backward of the norm ----
 struct BwdPlan {
-    enum { WIDE, REGISTERS, RING } kind;   // rows beyond a CTA's registers; the next row in registers; rows in shared memory
+    enum { WIDE, NARROW, RING } kind;      // rows beyond a CTA's registers; less than a warp a row; rows in shared memory
     int per;                               // values a thread
     int group, groups;                     // threads a row, rows at a time in a CTA
     long long parts;                       // partial rows
 };
 
+// A row of the ring in shared memory; ragged ones have up to 15 bytes in front, and are read 16 bytes beyond their end.
+size_t ring_slot(int64_t width, int size, bool aligned) {
+    return aligned ? (size_t)width * size : ((size_t)width * size + 15) / 16 * 16 + 32;
+}
 // shared memory beside the rows: the weight, the barriers, their alignment
-size_t ring_rest(int64_t width) { return (size_t)width * 4 + 15 * 4 * 8 + 256; }
-int ring_stages(int64_t width, int groups, int size, int tensors, const DevInfo& d) {
-    const size_t row = tensors * (size_t)width * size * groups, rest = ring_rest(width) + 1024;
+size_t ring_rest(int64_t width) { return (size_t)(width + 8) * 4 + 15 * 4 * 8 + 256; }
+int ring_stages(int64_t width, int groups, int size, int tensors, bool aligned, const DevInfo& d) {
+    const size_t row = tensors * ring_slot(width, size, aligned) * groups, rest = ring_rest(width) + 1024;
     const long long n = (long long)d.max_smem > (long long)rest ? (long long)((d.max_smem - rest) / row) : 0;
     return (int)(n < 4 ? n : 4);
 }
@@ -114,7 +118,7 @@ BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, 
     }
     const auto threads = [&](int per) { return (int)(((width + per - 1) / per + 31) / 32 * 32); };
     const int tensors = add ? 3 : 2;
-    if (aligned && width > 128) {
+    if (width > 128) {
         // The form that leaves the fewest threads without values: 8, 16 or 24 values a thread, of which an SM's registers
         // hold 640, 512 and 384 threads.  Fewer values a thread cost more for what each row takes beside them, and a row at
         // a time leaves its reduction uncovered.  bf16, GB/s by values a thread, 8 / 16 / 24: width 512 4000 / 5170 / 4560,
@@ -124,8 +128,8 @@ BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, 
         for (int per : {16, 24, 8}) {
             const int group = threads(per), most = per == 24 ? 384 : per == 8 ? 640 : 512;
             int groups = most / group < 15 ? most / group : 15;      // named barriers
-            while (groups > 1 && ring_stages(width, groups, size, tensors, d) < 3) --groups;
-            if (groups == 0 || ring_stages(width, groups, size, tensors, d) < 2) continue;
+            while (groups > 1 && ring_stages(width, groups, size, tensors, aligned, d) < 3) --groups;
+            if (groups == 0 || ring_stages(width, groups, size, tensors, aligned, d) < 2) continue;
             const double score = (double)width * groups / ((double)per * most) * (per == 8 ? 0.85 : 1.0) * (groups > 1 ? 1.0 : 0.8);
             if (score <= best) continue;
             best = score;
@@ -134,12 +138,16 @@ BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, 
             b.groups = groups;
         }
     }
-    if (b.per == 0) {
-        b.kind = BwdPlan::REGISTERS;
-        b.per = width <= 2048 ? 8 : 16;
-        const int n = (int)((width + b.per - 1) / b.per);
-        b.group = n <= 8 ? 8 : n <= 16 ? 16 : threads(b.per);
-        b.groups = b.group < 32 ? 512 / 32 * (32 / b.group) : 512 / b.group < 15 ? 512 / b.group : 15;
+    if (width > 128 && b.per == 0) {      // shared memory for less than two rows (not on a B200)
+        b.kind = BwdPlan::WIDE;
+        b.parts = bwd_parts(rows, width, d.sms);
+        return b;
+    }
+    if (width <= 128) {
+        b.kind = BwdPlan::NARROW;
+        b.per = 8;
+        b.group = width <= 64 ? 8 : 16;
+        b.groups = 512 / b.group;
     }
     if (b.group >= 32) {
         // few rows: over all SMs first
@@ -164,60 +172,36 @@ int allow_smem(int bytes) {
     return MAM_OK;
 }
 
-template <typename T, int NV, bool ADD, int MODE>
+template <auto KERNEL>
 int ring_run(const NormBwdParams& p, const BwdPlan& b, const BwdRing& r, cudaStream_t st) {
-    const int e = allow_smem<mam_norm_bwd_ring_kernel<T, NV, ADD, MODE>>((int)r.bytes);
+    const int e = allow_smem<KERNEL>((int)r.bytes);
     if (e != MAM_OK) return e;
-    mam_norm_bwd_ring_kernel<T, NV, ADD, MODE><<<(unsigned)b.parts, b.group * b.groups, r.bytes, st>>>(p, r);
+    KERNEL<<<(unsigned)b.parts, b.group * b.groups, r.bytes, st>>>(p, r);
     MAM_CUDA(cudaGetLastError());
     return MAM_OK;
 }
 template <typename T, int NV, bool ADD>
-int ring_launch(const NormBwdParams& p, const BwdPlan& b, const DevInfo& d, cudaStream_t st) {
+int ring_launch(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
     BwdRing r{};
     r.group = b.group;
     r.groups = b.groups;
-    r.row_bytes = (unsigned)(p.width * sizeof(T));
-    r.stages = ring_stages(p.width, b.groups, sizeof(T), ADD ? 3 : 2, d);
+    r.slot_bytes = (unsigned)ring_slot(p.width, sizeof(T), aligned);
+    r.stages = ring_stages(p.width, b.groups, sizeof(T), ADD ? 3 : 2, aligned, d);
     if (r.stages < 2) return MAM_ERR_UNSUPPORTED;
-    const size_t row = (ADD ? 3 : 2) * (size_t)r.row_bytes * b.groups;
+    const size_t row = (ADD ? 3 : 2) * (size_t)r.slot_bytes * b.groups;
     r.weights_at = (unsigned)((row * r.stages + 127) / 128 * 128);
-    r.bars_at = (unsigned)(r.weights_at + (p.width * 4 + 15) / 16 * 16);
+    r.bars_at = (unsigned)(r.weights_at + (p.width + VEC<T> - 1) / VEC<T> * VEC<T> * 4);
     r.bytes = r.bars_at + b.groups * r.stages * 8;
-    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<T, NV, ADD, FULL>(p, b, r, st);
-    return ring_run<T, NV, ADD, ALIGNED>(p, b, r, st);
+    if (!aligned) return ring_run<mam_norm_bwd_ragged_kernel<T, NV, ADD>>(p, b, r, st);
+    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, FULL>>(p, b, r, st);
+    return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, b, r, st);
 }
 
-template <typename T, int NV, bool ADD, int MODE, int LANES>
-int bwd_run(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
-    const int rows = b.group < 32 ? b.group * b.groups / 32 : b.groups;
-    const size_t smem = rows > 1 ? (size_t)rows * 2 * (size_t)p.width * 4 : 0;
-    if (smem > 40 * 1024) {
-        const int e = allow_smem<mam_norm_bwd_kernel<T, NV, ADD, MODE, LANES>>((int)smem);
-        if (e != MAM_OK) return e;
-    }
-    mam_norm_bwd_kernel<T, NV, ADD, MODE, LANES><<<(unsigned)b.parts, b.group * b.groups, smem, st>>>(p, b.group);
-    MAM_CUDA(cudaGetLastError());
-    return MAM_OK;
-}
-template <typename T, int NV, bool ADD, int MODE>
-int bwd_launch(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
-    if constexpr (MODE == RAGGED) {
-        if (b.group >= 32) return bwd_run<T, NV, ADD, MODE, 32>(p, b, st);
-    }
-    if constexpr (NV * VEC<T> == 8) {
-        if (b.group == 8) return bwd_run<T, NV, ADD, MODE, 8>(p, b, st);
-        return bwd_run<T, NV, ADD, MODE, 16>(p, b, st);
-    }
-    return MAM_ERR_UNSUPPORTED;
-}
-template <typename T, int NV, bool ADD>
-int bwd_mode(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
-    if (b.kind == BwdPlan::RING) return ring_launch<T, NV, ADD>(p, b, d, st);
-    if constexpr (NV * VEC<T> != 24)
-        if (!aligned || b.group >= 32) return bwd_launch<T, NV, ADD, RAGGED>(p, b, st);
-    if constexpr (NV * VEC<T> == 8) return bwd_launch<T, NV, ADD, ALIGNED>(p, b, st);   // narrow rows
-    return MAM_ERR_UNSUPPORTED;
+template <typename T, bool ADD, int MODE>
+void narrow_launch(const NormBwdParams& p, const BwdPlan& b, cudaStream_t st) {
+    const size_t smem = 16 * 2 * (size_t)p.width * 4;      // at most 16 KB
+    if (b.group == 8) mam_norm_bwd_narrow_kernel<T, 8 / VEC<T>, ADD, MODE, 8><<<(unsigned)b.parts, 512, smem, st>>>(p);
+    else mam_norm_bwd_narrow_kernel<T, 8 / VEC<T>, ADD, MODE, 16><<<(unsigned)b.parts, 512, smem, st>>>(p);
 }
 
 template <typename T, bool ADD, int MODE>
@@ -231,10 +215,16 @@ void wide_launch(const NormBwdParams& p, cudaStream_t st) {
 
 template <typename T, bool ADD>
 int bwd_pick(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
-    if (b.kind != BwdPlan::WIDE) {
-        if (b.per == 8) return bwd_mode<T, 8 / VEC<T>, ADD>(p, b, aligned, d, st);
-        if (b.per == 16) return bwd_mode<T, 16 / VEC<T>, ADD>(p, b, aligned, d, st);
-        return bwd_mode<T, 24 / VEC<T>, ADD>(p, b, aligned, d, st);
+    if (b.kind == BwdPlan::RING) {
+        if (b.per == 8) return ring_launch<T, 8 / VEC<T>, ADD>(p, b, aligned, d, st);
+        if (b.per == 16) return ring_launch<T, 16 / VEC<T>, ADD>(p, b, aligned, d, st);
+        return ring_launch<T, 24 / VEC<T>, ADD>(p, b, aligned, d, st);
+    }
+    if (b.kind == BwdPlan::NARROW) {
+        if (aligned) narrow_launch<T, ADD, ALIGNED>(p, b, st);
+        else narrow_launch<T, ADD, RAGGED>(p, b, st);
+        MAM_CUDA(cudaGetLastError());
+        return MAM_OK;
     }
     if (aligned) wide_launch<T, ADD, ALIGNED>(p, st);
     else wide_launch<T, ADD, RAGGED>(p, st);

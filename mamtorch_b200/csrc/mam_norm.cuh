@@ -278,23 +278,17 @@ __global__ void __launch_bounds__(1024) mam_norm_fwd_wide_kernel(const __grid_co
     }
 }
 
-// Backward of rows of up to NV vectors a thread.  blockDim.x / group groups of `group` threads (8, 16 or a multiple of 32)
-// walk the rows; a thread keeps its columns' sums of gy h and gy in registers over all of them, and the CTA leaves one
-// partial row of each.  The next row's vectors are on their way while a row is reduced.
+// Backward of narrow rows, of up to LANES (8 or 16) times NV vectors: 512 / LANES rows at a time in a CTA.  A thread keeps its
+// columns' sums of gy h and gy in registers over all its rows, and the CTA leaves one partial row of each.  The next row's
+// vectors are on their way while a row is reduced.
 template <typename T, int NV, bool ADD, int MODE, int LANES>
-__global__ void __launch_bounds__(512)
-mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
-    extern __shared__ float cols[];    // [groups][2][width] at the end
-    __shared__ float2 slot[2][32];
-    constexpr int V = VEC<T>, nt = LANES, MOST = 16;    // warps a CTA can have
-    if (LANES < 32) group = LANES;
-    const int groups = blockDim.x / group, g = threadIdx.x / group, t = threadIdx.x % group;
-    const int lane = threadIdx.x & 31, tl = t & (nt - 1);
-    const int warps = group >> 5, slot0 = (g * group) >> 5;
-    const int width = (int)p.width;
-    const int first = (t >> 5) * NV * 32 * V + tl * V;    // a warp's vectors follow one another
-    auto col = [&](int i) { return first + i * nt * V; };
-    auto count = [&](int i) { return MODE == FULL ? V : min(V, width - col(i)); };
+__global__ void __launch_bounds__(512) mam_norm_bwd_narrow_kernel(const __grid_constant__ NormBwdParams p) {
+    extern __shared__ float cols[];    // [warps][2][width] at the end
+    constexpr int V = VEC<T>;
+    const int g = threadIdx.x / LANES, t = threadIdx.x % LANES, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int width = (int)p.width, first = t * V;
+    auto col = [&](int i) { return first + i * LANES * V; };
+    auto count = [&](int i) { return min(V, width - col(i)); };
     uint4 carry = make_uint4(0u, 0u, 0u, 0u), carry2 = carry;
     float2 w[NV][V / 2], aw[NV][V / 2], ab[NV][V / 2];
 #pragma unroll
@@ -304,8 +298,7 @@ mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
         for (int j = 0; j < V / 2; ++j) aw[i][j] = ab[i][j] = splat2(0.f);
     }
     const float inv_n = p.inv_width;
-    // groups of less than a warp keep step with their warp
-    const int g0 = LANES < 32 ? (threadIdx.x >> 5) * (32 / LANES) : g;
+    const int groups = 512 / LANES, g0 = warp * (32 / LANES);      // the rows of a warp keep step
     const long long step = (long long)gridDim.x * groups;
     const bool has_gy = p.gy != nullptr, has_gs = ADD && p.gs != nullptr, has_dx = ADD && p.dx != nullptr;
     const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy), *gs0 = static_cast<const T*>(p.gs);
@@ -332,9 +325,8 @@ mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) qg[i] = make_uint4(0u, 0u, 0u, 0u);
     fetch();
-    int parity = 0;
     for (; base < p.rows; base += step) {
-        const bool valid = LANES == 32 || ahead < p.rows;
+        const bool valid = ahead < p.rows;
         const long long row_at = at;
         const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
         const float rstd = st.y;
@@ -375,16 +367,7 @@ mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
                     s2 = fma2(a[i][j], h[i][j], s2);
                 }
             }
-        float2 m = lane_sum2<LANES>(sum2(s1), sum2(s2));
-        if (LANES == 32 && warps > 1) {
-            // two sets of slots in turn: a set is written again only behind the next row's barrier
-            if (lane == 0) slot[parity][threadIdx.x >> 5] = m;
-            asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
-            const int k = lane & (MOST - 1);
-            m = k < warps ? slot[parity][slot0 + k] : make_float2(0.f, 0.f);
-            m = lane_sum2<MOST>(m.x, m.y);
-            parity ^= 1;
-        }
+        const float2 m = lane_sum2<LANES>(sum2(s1), sum2(s2));
         // ds = r a - (r mean(a) + h r mean(a h))
         const float2 c1 = splat2(-rstd * (m.x * inv_n)), c2 = splat2(-rstd * (m.y * inv_n));
         const bool odd = MODE == RAGGED && ((row_at + first) & 1);
@@ -409,24 +392,23 @@ mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
                 q = pack<T>(d);
                 if constexpr (ADD) {
                     if (has_dx) {
-                        mam_drop_pairs<V / 2>(d, start + (unsigned long long)(i * nt * (V / 2)) * MAM_DROP_STEP, odd,
+                        mam_drop_pairs<V / 2>(d, start + (unsigned long long)(i * LANES * (V / 2)) * MAM_DROP_STEP, odd,
                                               p.drop.threshold, p.drop.scale);
                         qd = pack<T>(d);
                     }
                 }
             }
-            store_vec<T, MODE>(ds + col(i), q, rest, tl, nt, i == 0, i == NV - 1, carry);
+            store_vec<T, MODE>(ds + col(i), q, rest, t, LANES, i == 0, i == NV - 1, carry);
             if constexpr (ADD) {
-                if (has_dx) store_vec<T, MODE>(dx + col(i), qd, rest, tl, nt, i == 0, i == NV - 1, carry2);
+                if (has_dx) store_vec<T, MODE>(dx + col(i), qd, rest, t, LANES, i == 0, i == NV - 1, carry2);
             }
         }
         start += drop_step;
     }
     if (!p.partial) return;
     float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
-    // groups of one warp are added by shuffles, the rest in shared memory: a fixed order
-    const int rows = LANES < 32 ? (int)blockDim.x >> 5 : groups, mine = LANES < 32 ? (int)threadIdx.x >> 5 : g;
-    float* to = rows > 1 ? cols + (size_t)mine * 2 * width : out;
+    // the rows of a warp are added by shuffles, the warps in shared memory: a fixed order
+    float* to = cols + (size_t)warp * 2 * width;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float f[2][V];
@@ -440,27 +422,27 @@ mam_norm_bwd_kernel(const __grid_constant__ NormBwdParams p, int group) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 if (LANES == 8) f[k][j] += __shfl_xor_sync(~0u, f[k][j], 8);
-                if (LANES < 32) f[k][j] += __shfl_xor_sync(~0u, f[k][j], 16);
-                if (col(i) + j < width && (LANES == 32 || lane < LANES)) to[k * width + col(i) + j] = f[k][j];
+                f[k][j] += __shfl_xor_sync(~0u, f[k][j], 16);
+                if (col(i) + j < width && lane < LANES) to[k * width + col(i) + j] = f[k][j];
             }
     }
-    if (rows == 1) return;
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
+    for (int c = threadIdx.x; c < 2 * width; c += 512) {
         float sum = cols[c];
-        for (int k = 1; k < rows; ++k) sum += cols[(size_t)k * 2 * width + c];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) sum += cols[(size_t)k * 2 * width + c];
         out[c] = sum;
     }
 }
 
-// The same for aligned rows from a warp's width on, with the rows brought to shared memory by bulk copies: `stages` rows of
-// each group are there or on their way, whatever the registers leave room for.  With the next row's vectors in
-// registers instead, [16384, 5120] bf16 with dropout took 289 us and [32768, 4096] 336.
+// The same for rows from a warp's width on, with the rows brought to shared memory by bulk copies: `stages` rows of each group
+// of `group` threads (whole warps) are there or on their way, whatever the registers leave room for.  With the next row's
+// vectors in registers instead, bf16 [32768, 4096] took 155 us (this: 130) and with dropout 336 (211).
 // A row's stage is free when its group has passed the next row's barrier; thread 0 of the group then sends for the row
 // `stages - 1` ahead.
 struct BwdRing {
     int group, groups, stages;
-    unsigned row_bytes;         // of one tensor's row
+    unsigned slot_bytes;                   // of one tensor's row
     unsigned weights_at, bars_at, bytes;   // places in shared memory, and its size
 };
 
@@ -479,7 +461,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
     const bool has_gy = p.gy != nullptr, has_gs = ADD && p.gs != nullptr, has_dx = ADD && p.dx != nullptr;
     const int tensors = 1 + has_gy + has_gs;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring.bars_at) + g * ring.stages;
-    unsigned char* mine = smem + (size_t)g * ring.stages * TENSORS * ring.row_bytes;      // [stage][s, gy, gs][row]
+    unsigned char* mine = smem + (size_t)g * ring.stages * TENSORS * ring.slot_bytes;      // [stage][s, gy, gs][row]
     // the weight in fp32, the halves of a vector of eight apart: a warp's 16-byte reads then meet no bank twice
     float4* weights = reinterpret_cast<float4*>(smem + ring.weights_at);
     const int vecs = (width + V - 1) / V;
@@ -500,11 +482,11 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
     const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy), *gs0 = static_cast<const T*>(p.gs);
     auto send = [&](long long row, int stage) {
         if (row >= p.rows) return;
-        unsigned char* to = mine + (size_t)stage * TENSORS * ring.row_bytes;
-        mbar_expect_tx(full + stage, tensors * ring.row_bytes);
-        bulk_load(to, s0 + row * p.s_pitch, ring.row_bytes, full + stage);
-        if (has_gy) bulk_load(to + ring.row_bytes, gy0 + row * p.width, ring.row_bytes, full + stage);
-        if (has_gs) bulk_load(to + 2 * ring.row_bytes, gs0 + row * p.width, ring.row_bytes, full + stage);
+        unsigned char* to = mine + (size_t)stage * TENSORS * ring.slot_bytes;
+        mbar_expect_tx(full + stage, tensors * ring.slot_bytes);
+        bulk_load(to, s0 + row * p.s_pitch, ring.slot_bytes, full + stage);
+        if (has_gy) bulk_load(to + ring.slot_bytes, gy0 + row * p.width, ring.slot_bytes, full + stage);
+        if (has_gs) bulk_load(to + 2 * ring.slot_bytes, gs0 + row * p.width, ring.slot_bytes, full + stage);
     };
     long long row = (long long)blockIdx.x * groups + g;
     if (t == 0)
@@ -528,7 +510,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
         const float2 st = next;
         if (row + step < p.rows) next = p.stats[row + step];
         const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
-        const unsigned char* from = mine + (size_t)stage * TENSORS * ring.row_bytes;
+        const unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
         if (!mbar_wait_bounded(full + stage, phase, lost ? 1024 : 1u << 22)) {
             lost = true;            // the results are void, but every barrier is still met and every copy waited for
             *p.wait_flag = 1;
@@ -540,7 +522,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
                 const uint4* q = reinterpret_cast<const uint4*>(from) + vec0 + i * 32;
                 unpack<T>(*q, h[i]);
                 if (has_gy) {
-                    unpack<T>(*reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(q) + ring.row_bytes), a[i]);
+                    unpack<T>(*reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned char*>(q) + ring.slot_bytes), a[i]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < V / 2; ++j) a[i][j] = splat2(0.f);
@@ -588,7 +570,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
                 if constexpr (ADD) {
                     if (has_gs) {
                         Vals<T> f;
-                        unpack<T>(*(reinterpret_cast<const uint4*>(from + 2 * ring.row_bytes) + vec0 + i * 32), f);
+                        unpack<T>(*(reinterpret_cast<const uint4*>(from + 2 * ring.slot_bytes) + vec0 + i * 32), f);
 #pragma unroll
                         for (int j = 0; j < V / 2; ++j) d[j] = add2(d[j], f[j]);
                     }
@@ -622,6 +604,221 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
                 *reinterpret_cast<float2*>(to + width + col(i) + 2 * j) = ab[i][j];
             }
         }
+    if (groups == 1) return;
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
+        float sum = cols[c];
+        for (int k = 1; k < groups; ++k) sum += cols[(size_t)k * 2 * width + c];
+        out[c] = sum;
+    }
+}
+
+// The ring for rows that are not 16-byte aligned.  They are copied with the aligned 16 bytes at either end, which belong to
+// the rows beside them; the first and the last row have no such neighbours and are brought element by element.  A thread
+// shifts its vectors out of two aligned ones, and the stores take the way of ragged rows.  (A kernel of its own: as one
+// template the aligned form lost 3 to 8 %.)  bf16 [5003, 1283] 25 us, with the next row's vectors in registers instead 40.
+template <typename T, int NV, bool ADD>
+__global__ void __launch_bounds__(NV * VEC<T> == 8 ? 640 : NV * VEC<T> == 24 ? 384 : 512)
+mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid_constant__ BwdRing ring) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float2 slot[2][32];
+    constexpr int V = VEC<T>, HALVES = V / 4, TENSORS = ADD ? 3 : 2, MOST = NV * V == 8 ? 32 : 16;      // warps a group can have
+    const int group = ring.group, groups = ring.groups, g = threadIdx.x / group, t = threadIdx.x - g * group;
+    const int lane = threadIdx.x & 31, warps = group >> 5, slot0 = (g * group) >> 5;
+    const int width = (int)p.width;
+    const int vec0 = (t >> 5) * NV * 32 + lane;     // a warp's vectors follow one another
+    auto col = [&](int i) { return (vec0 + i * 32) * V; };
+    auto count = [&](int i) { return min(V, width - col(i)); };
+    const bool has_gy = p.gy != nullptr, has_gs = ADD && p.gs != nullptr, has_dx = ADD && p.dx != nullptr;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring.bars_at) + g * ring.stages;
+    unsigned char* mine = smem + (size_t)g * ring.stages * TENSORS * ring.slot_bytes;      // [stage][s, gy, gs][row]
+    // the weight in fp32, the halves of a vector of eight apart: a warp's 16-byte reads then meet no bank twice
+    float4* weights = reinterpret_cast<float4*>(smem + ring.weights_at);
+    const int vecs = (width + V - 1) / V;
+    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+        float2 w[V / 2];
+        load_param<T, RAGGED>(p.weight, p.params_f32, v * V, min(V, width - v * V), 1.f, w);
+#pragma unroll
+        for (int k = 0; k < HALVES; ++k)
+            weights[k * vecs + v] = make_float4(w[2 * k].x, w[2 * k].y, w[2 * k + 1].x, w[2 * k + 1].y);
+    }
+    if (t == 0) {
+        for (int k = 0; k < ring.stages; ++k) mbar_init(full + k, 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+
+    const long long step = (long long)gridDim.x * groups;
+    const T *s0 = static_cast<const T*>(p.s), *gy0 = static_cast<const T*>(p.gy), *gs0 = static_cast<const T*>(p.gs);
+    const unsigned row_bytes = (unsigned)width * sizeof(T);
+    auto misfit = [](const T* q) { return (unsigned)(reinterpret_cast<uintptr_t>(q) & 15u); };
+    auto edge = [&](long long row) { return row == 0 || row == p.rows - 1; };
+    auto send = [&](long long row, int stage) {
+        if (row >= p.rows) return;
+        if (edge(row)) {
+            mbar_arrive(full + stage);
+            return;
+        }
+        unsigned char* to = mine + (size_t)stage * TENSORS * ring.slot_bytes;
+        const T* from[3] = {s0 + row * p.s_pitch, gy0 + row * p.width, gs0 + row * p.width};
+        const bool has[3] = {true, has_gy, has_gs};
+        unsigned bytes[3], all = 0;
+#pragma unroll
+        for (int k = 0; k < TENSORS; ++k) {
+            bytes[k] = (misfit(from[k]) + row_bytes + 15u) & ~15u;
+            if (has[k]) all += bytes[k];
+        }
+        mbar_expect_tx(full + stage, all);
+#pragma unroll
+        for (int k = 0; k < TENSORS; ++k)
+            if (has[k])
+                bulk_load(to + k * ring.slot_bytes, reinterpret_cast<const unsigned char*>(from[k]) - misfit(from[k]), bytes[k],
+                          full + stage);
+    };
+    long long row = (long long)blockIdx.x * groups + g;
+    if (t == 0)
+        for (int k = 0; k < ring.stages - 1; ++k) send(row + k * step, k);
+
+    float2 aw[NV][V / 2], ab[NV][V / 2];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) aw[i][j] = ab[i][j] = splat2(0.f);
+    const float inv_n = p.inv_width;
+    long long at = row * p.width;
+    const long long at_step = step * p.width;
+    const unsigned long long seed = has_dx ? p.drop.seed_now() : 0;
+    float2 next = row < p.rows ? p.stats[row] : make_float2(0.f, 0.f);
+    uint4 carry = make_uint4(0u, 0u, 0u, 0u), carry2 = carry;
+    int stage = 0;
+    unsigned phase = 0, parity = 0;
+    bool lost = false;
+    auto meet = [&]() {
+        if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
+        else __syncwarp();
+    };
+    for (; row < p.rows; row += step, at += at_step) {
+        const float2 st = next;
+        if (row + step < p.rows) next = p.stats[row + step];
+        const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
+        unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
+        if (!mbar_wait_bounded(full + stage, phase, lost ? 1024 : 1u << 22)) {
+            lost = true;            // the results are void, but every barrier is still met and every copy waited for
+            *p.wait_flag = 1;
+        }
+        const T *ps = s0 + row * p.s_pitch, *py = gy0 + at, *pz = gs0 + at;
+        if (edge(row)) {
+            T *ds = reinterpret_cast<T*>(from + misfit(ps)), *dy = reinterpret_cast<T*>(from + ring.slot_bytes + misfit(py)),
+              *dz = reinterpret_cast<T*>(from + 2 * ring.slot_bytes + misfit(pz));
+            for (int c = t; c < width; c += group) {
+                ds[c] = ps[c];
+                if (has_gy) dy[c] = py[c];
+                if (has_gs) dz[c] = pz[c];
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // before a later copy into this stage
+            meet();
+        }
+        auto vector = [&](int tensor, const T* src, int i) {
+            const uint4* q = reinterpret_cast<const uint4*>(from + tensor * ring.slot_bytes) + vec0 + i * 32;
+            return cut<T>(q[0], q[1], misfit(src));
+        };
+        float2 h[NV][V / 2], a[NV][V / 2], s1 = splat2(0.f), s2 = s1;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (count(i) > 0) {
+                unpack<T>(vector(0, ps, i), h[i]);
+                if (has_gy) {
+                    unpack<T>(vector(1, py, i), a[i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V / 2; ++j) a[i][j] = splat2(0.f);
+                }
+                float2 w[V / 2];
+#pragma unroll
+                for (int k = 0; k < HALVES; ++k) {
+                    const float4 f = weights[k * vecs + vec0 + i * 32];
+                    w[2 * k] = make_float2(f.x, f.y);
+                    w[2 * k + 1] = make_float2(f.z, f.w);
+                }
+                if (count(i) < V) {
+                    keep_first<T>(h[i], count(i));
+                    keep_first<T>(a[i], count(i));
+                }
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    h[i][j] = mul2(add2(h[i][j], minus), r2);
+                    aw[i][j] = fma2(a[i][j], h[i][j], aw[i][j]);
+                    ab[i][j] = add2(ab[i][j], a[i][j]);
+                    a[i][j] = mul2(a[i][j], w[j]);
+                    s1 = add2(s1, a[i][j]);
+                    s2 = fma2(a[i][j], h[i][j], s2);
+                }
+            }
+        float2 m = lane_sum2<32>(sum2(s1), sum2(s2));
+        // two sets of slots in turn: a set is written again only behind the next row's barrier
+        if (warps > 1 && lane == 0) slot[parity][threadIdx.x >> 5] = m;
+        meet();
+        // all have left the row before this one: its stage takes the row stages - 1 ahead
+        if (t == 0) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
+        if (warps > 1) {
+            m = (lane & (MOST - 1)) < warps ? slot[parity][slot0 + (lane & (MOST - 1))] : make_float2(0.f, 0.f);
+            m = lane_sum2<MOST>(m.x, m.y);
+            parity ^= 1;
+        }
+        // ds = r a - (r mean(a) + h r mean(a h))
+        const float2 c1 = splat2(-st.y * (m.x * inv_n)), c2 = splat2(-st.y * (m.y * inv_n));
+        const unsigned long long start = mam_drop_start(seed, at + vec0 * V);
+        const bool odd = (at + vec0 * V) & 1;
+        T *ds = static_cast<T*>(p.ds) + at, *dx = static_cast<T*>(p.dx) + at;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            uint4 q = make_uint4(0u, 0u, 0u, 0u), qd = q;
+            if (count(i) > 0) {
+                Vals<T> d;
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) d[j] = fma2(a[i][j], r2, fma2(h[i][j], c2, c1));
+                if constexpr (ADD) {
+                    if (has_gs) {
+                        Vals<T> f;
+                        unpack<T>(vector(2, pz, i), f);
+#pragma unroll
+                        for (int j = 0; j < V / 2; ++j) d[j] = add2(d[j], f[j]);
+                    }
+                }
+                q = pack<T>(d);
+                if constexpr (ADD) {
+                    if (has_dx) {
+                        mam_drop_pairs<V / 2>(d, start + (unsigned long long)(i * 32 * (V / 2)) * MAM_DROP_STEP, odd,
+                                              p.drop.threshold, p.drop.scale);
+                        qd = pack<T>(d);
+                    }
+                }
+            }
+            const int rest = width - col(i);
+            store_vec<T, RAGGED>(ds + col(i), q, rest, lane, 32, i == 0, i == NV - 1, carry);
+            if constexpr (ADD) {
+                if (has_dx) store_vec<T, RAGGED>(dx + col(i), qd, rest, lane, 32, i == 0, i == NV - 1, carry2);
+            }
+        }
+        if (++stage == ring.stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+    if (!p.partial) return;
+    float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
+    // the groups' sums meet in the ring's memory, where no copy is on its way any more: a fixed order
+    __syncthreads();
+    float* cols = reinterpret_cast<float*>(smem);
+    float* to = groups > 1 ? cols + (size_t)g * 2 * width : out;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (col(i) + j < width) {
+                to[col(i) + j] = j & 1 ? aw[i][j / 2].y : aw[i][j / 2].x;
+                to[width + col(i) + j] = j & 1 ? ab[i][j / 2].y : ab[i][j / 2].x;
+            }
     if (groups == 1) return;
     __syncthreads();
     for (int c = threadIdx.x; c < 2 * width; c += blockDim.x) {
