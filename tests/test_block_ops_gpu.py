@@ -746,3 +746,70 @@ def test_captured_block_drops_anew_at_each_replay(cuda):
         share = (y == x).double().mean().item()
         assert abs(share - 0.5) < 6 * 0.5 / math.sqrt(x.numel())
     assert torch.isfinite(step.grad_input).all()
+
+
+# ---------------------------------------------------------------- torch around them
+
+def test_schemas_and_shape_functions(cuda):
+    from torch.library import opcheck
+
+    import mamtorch_b200  # noqa: F401
+
+    ops = torch.ops.mamtorch_b200
+    x, r = (inputs((6, 5, 40), torch.bfloat16, k, cuda) for k in (1, 2))
+    w, b = params(40, torch.float32, 3, cuda)
+    at = torch.tensor([5], device=cuda)
+    stats = torch.rand(30, 2, device=cuda)
+    for op, args in ((ops.layer_norm_forward, (x, None, w, b, 1e-5, 0.0, 0, None, True)),
+                     (ops.layer_norm_forward, (x, r, None, None, 1e-5, 0.1, 3, at, False)),
+                     (ops.layer_norm_backward, (x, r, x, stats, w, 0.1, 3, None, True, True, True)),
+                     (ops.layer_norm_backward, (x, None, x, stats, w, 0.0, 0, None, True, False, True)),
+                     (ops.dropout_forward, (x, r, 0.1, 3, at)), (ops.gelu_forward, (x, 0.1, 3, None)),
+                     (ops.gelu_backward, (r, x, 0.1, 3, None))):
+        opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
+
+
+def test_traced_checkpointed_and_transformed_calls(cuda):
+    import torch.utils.checkpoint as checkpoint
+
+    from mamtorch_b200.nn import functional as MF
+
+    x = inputs((16, 64), torch.float32, 1, cuda).requires_grad_()
+    w, b = (p.requires_grad_() for p in params(64, torch.float32, 2, cuda))
+
+    def f(x, w, b):
+        y, s = MF.dropout_add_layer_norm(MF.gelu(x, 0.1, 3), x, w, b, 1e-5, 0.1, 7)
+        return y * s
+
+    want = f(x, w, b)
+    grads = torch.autograd.grad(want.sum(), (x, w, b))
+    got = torch.compile(f, backend="aot_eager")(x, w, b)
+    assert torch.equal(got, want)
+    for p, q in zip(torch.autograd.grad(got.sum(), (x, w, b)), grads):
+        assert torch.allclose(p, q, rtol=1e-5, atol=1e-5 * q.abs().max().item())
+    # a recomputed forward draws the same numbers, from the restored generator
+    drop = lambda v: MF.dropout(MF.gelu(v, 0.3), 0.3)   # noqa: E731
+    torch.manual_seed(1)
+    y = checkpoint.checkpoint(drop, x, use_reentrant=False)
+    (a,) = torch.autograd.grad(y.sum(), x)
+    torch.manual_seed(1)
+    z = drop(x)
+    assert torch.equal(y, z) and torch.equal(a, torch.autograd.grad(z.sum(), x)[0])
+    (a,) = torch.autograd.grad(MF.gelu(x).square().sum(), x)
+    assert torch.equal(torch.func.grad(lambda v: MF.gelu(v).square().sum())(x.detach()), a)
+
+
+def test_saved_tensors_are_guarded(cuda):
+    from mamtorch_b200.nn import functional as MF
+
+    x = inputs((16, 64), torch.float32, 1, cuda).requires_grad_()
+    y, s = MF.dropout_add_layer_norm(x * 2, x)
+    s.data  # reading is fine
+    with torch.no_grad():
+        s.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = MF.layer_norm(x)
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
