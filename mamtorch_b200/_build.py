@@ -1,7 +1,7 @@
 """In-tree build of the two native pieces of this package.
 
   libmam_b200.so  the CUDA kernels behind a plain C ABI (nvcc, sm_100a only)
-  _C.so           the PyTorch operator shim (g++), linked against libmam_b200.so
+  _C.so           the PyTorch operator shim (g++), linked against libmam_b200.so; also the Python module `_C`
 
 Both land next to this file so they travel with the source tree; nothing is installed into
 site-packages and nothing is built lazily at import time on a machine without the sources.
@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -62,14 +63,14 @@ def build_shim(force: bool = False) -> str:
         import torch
         from torch.utils import cpp_extension as ce
 
-        inc = []
+        inc = ["-I", sysconfig.get_paths()["include"]]
         for p in ce.include_paths("cuda"):
             inc += ["-I", p]
         tlib = os.path.join(os.path.dirname(torch.__file__), "lib")
         cxx = "g++"
-        cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-o", SHIM, *srcs, *inc,
+        cmd = [cxx, "-O2", "-DTORCH_EXTENSION_NAME=_C", "-std=c++17", "-fPIC", "-shared", "-o", SHIM, *srcs, *inc,
                "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),
-               "-L", tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
+               "-L", tlib, "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda", "-ltorch_python",
                "-L", HERE, "-l:libmam_b200.so",
                "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + tlib, "-Wno-deprecated-declarations"]
         subprocess.check_call(cmd, cwd=CSRC)

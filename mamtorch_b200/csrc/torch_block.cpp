@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 
 #include <vector>
@@ -411,4 +412,14 @@ TORCH_LIBRARY_IMPL(mamtorch_b200, CUDA, m) {
     m.impl("dropout_forward", &dropout_forward);
     m.impl("gelu_forward", &gelu_forward);
     m.impl("gelu_backward", &gelu_backward);
+}
+
+// The differentiable operators as plain functions of the module mamtorch_b200._C, for eager calls: the way through
+// torch.ops (a schema's arguments, boxed) takes a microsecond of the seven that a small call lasts.
+PYBIND11_MODULE(_C, m) {
+    const pybind11::call_guard<pybind11::gil_scoped_release> free;
+    m.def("layer_norm", &layer_norm, free);
+    m.def("dropout_add_layer_norm", &dropout_add_layer_norm, free);
+    m.def("dropout", &dropout, free);
+    m.def("gelu", &gelu, free);
 }

@@ -10,6 +10,8 @@ from __future__ import annotations
 import torch
 from torch import Tensor
 
+from .. import _C
+
 _ops = torch.ops.mamtorch_b200
 
 
@@ -427,6 +429,12 @@ def selection_count_update_(count: Tensor, argmax: Tensor, argmin: Tensor, hits=
 # after the tensor was advanced.  The backward reads it again, so it must not change between a forward and its backward
 # (autograd raises if it did).
 
+def _eager(x) -> bool:
+    """Whether the call may go to the C++ function itself: tracing and tensors with their own dispatch take the registered
+    operator, which does the same."""
+    return not (torch.compiler.is_compiling() or torch.overrides.has_torch_function_unary(x))
+
+
 def _drop_args(rate: float, seed):
     rate = float(rate)
     if not 0.0 <= rate < 1.0:
@@ -446,7 +454,7 @@ def _drop_args(rate: float, seed):
 def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
     """Layer norm over the last dimension.  Weight and bias are fp32 or have the dtype of x.  Rows that lie a constant
     distance apart (a slice of the last dimension) are read in place."""
-    return _ops.layer_norm.default(x, weight, bias, eps)
+    return (_C.layer_norm if _eager(x) else _ops.layer_norm.default)(x, weight, bias, eps)
 
 
 def dropout_add_layer_norm(x: Tensor, residual: Tensor, weight: Tensor | None = None, bias: Tensor | None = None,
@@ -454,16 +462,17 @@ def dropout_add_layer_norm(x: Tensor, residual: Tensor, weight: Tensor | None = 
     """(y, s): s = residual + dropout(x), the residual stream behind a block, and y = layer_norm(s), the input of the next.
     One pass forward and one backward; equal to `dropout(x, ..., residual)` followed by `layer_norm` bit for bit (the
     norm reads s as it is stored)."""
-    return _ops.dropout_add_layer_norm.default(x, residual, weight, bias, eps, *_drop_args(drop_rate, drop_seed))
+    f = _C.dropout_add_layer_norm if _eager(x) else _ops.dropout_add_layer_norm.default
+    return f(x, residual, weight, bias, eps, *_drop_args(drop_rate, drop_seed))
 
 
 def dropout(x: Tensor, drop_rate: float, drop_seed=None, residual: Tensor | None = None) -> Tensor:
     """dropout(x), or residual + dropout(x), the mask formed from the seed forward and backward and never stored.  It
     always drops (a training-time operator).  Its masks are not those of `weight_drop` and the MAM layers' output dropout:
     it takes one 64-bit draw for two elements, they take one for each."""
-    return _ops.dropout.default(x, residual, *_drop_args(drop_rate, drop_seed))
+    return (_C.dropout if _eager(x) else _ops.dropout.default)(x, residual, *_drop_args(drop_rate, drop_seed))
 
 
 def gelu(x: Tensor, drop_rate: float = 0.0, drop_seed=None) -> Tensor:
     """dropout(x * Phi(x)), Phi the integral of the normal distribution: the exact GELU, with the dropout behind it."""
-    return _ops.gelu.default(x, *_drop_args(drop_rate, drop_seed))
+    return (_C.gelu if _eager(x) else _ops.gelu.default)(x, *_drop_args(drop_rate, drop_seed))
