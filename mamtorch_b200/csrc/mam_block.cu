@@ -30,6 +30,51 @@ int drop_args(float rate, uint64_t seed, const int64_t* seed_at, DropArgs* d) {
     return MAM_OK;
 }
 
+// ---- rows through shared memory ----
+// A row of the ring in shared memory; ragged ones have up to 15 bytes in front, and are read 16 bytes beyond their end.
+size_t ring_slot(int64_t width, int size, bool aligned) {
+    return aligned ? (size_t)width * size : ((size_t)width * size + 15) / 16 * 16 + 32;
+}
+// shared memory beside the rows: the parameters, the barriers, their alignment
+size_t ring_rest(int64_t width, int params) { return params * (size_t)(width + 8) * 4 + 32 * 4 * 8 + 256; }
+int ring_stages(int64_t width, int groups, int size, int tensors, int params, bool aligned, const DevInfo& d) {
+    const size_t row = tensors * ring_slot(width, size, aligned) * groups, rest = ring_rest(width, params) + 1024;
+    const long long n = (long long)d.max_smem > (long long)rest ? (long long)((d.max_smem - rest) / row) : 0;
+    return (int)(n < 4 ? n : 4);
+}
+
+// Lets a kernel have `bytes` of dynamic shared memory; asked of the runtime once for each device and size that is larger.
+template <auto KERNEL>
+int allow_smem(int bytes) {
+    static std::atomic<int> allowed[64];
+    int dev = 0;
+    MAM_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
+    if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return MAM_OK;
+    MAM_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    allowed[dev].store(bytes, std::memory_order_relaxed);
+    return MAM_OK;
+}
+
+template <auto KERNEL, class Params>
+int ring_run(const Params& p, unsigned ctas, const NormRing& r, cudaStream_t st) {
+    const int e = allow_smem<KERNEL>((int)r.bytes);
+    if (e != MAM_OK) return e;
+    KERNEL<<<ctas, r.group * r.groups, r.bytes, st>>>(p, r);
+    MAM_CUDA(cudaGetLastError());
+    return MAM_OK;
+}
+NormRing ring_of(int64_t width, int group, int groups, int stages, int size, int tensors, int params, bool aligned) {
+    NormRing r{};
+    r.group = group;
+    r.groups = groups;
+    r.stages = stages;
+    r.slot_bytes = (unsigned)ring_slot(width, size, aligned);
+    r.weights_at = (unsigned)(((size_t)tensors * r.slot_bytes * groups * stages + 127) / 128 * 128);
+    r.bars_at = (unsigned)(r.weights_at + params * ((width + 7) / 8 * 8 * 4));
+    r.bytes = r.bars_at + groups * stages * 8;
+    return r;
+}
 // ---- forward of the norm ----
 template <typename T, int NV, bool ADD, int MODE>
 void fwd_launch(const NormFwdParams& p, int lanes, int threads, cudaStream_t st) {
@@ -53,12 +98,59 @@ void fwd_mode(const NormFwdParams& p, bool aligned, int lanes, int threads, cuda
     else fwd_launch<T, NV, ADD, ALIGNED>(p, lanes, threads, st);
 }
 
+// Threads a row and rows at a time for the forward's ring: the form that leaves the fewest threads without values.
+struct FwdPlan {
+    int per, group, groups;
+};
+FwdPlan fwd_plan(int64_t width, int size, bool add, bool aligned, const DevInfo& d) {
+    FwdPlan b{};
+    const int tensors = add ? 2 : 1;
+    double best = 0;
+    for (int per : {16, 24, 8}) {
+        const int group = (int)(((width + per - 1) / per + 31) / 32 * 32), most = per == 8 ? 1024 : per == 16 ? 768 : 640;
+        int groups = most / group;
+        if (group > 32 && groups > 15) groups = 15;      // named barriers
+        while (groups > 1 && ring_stages(width, groups, size, tensors, 2, aligned, d) < 3) --groups;
+        if (groups == 0 || ring_stages(width, groups, size, tensors, 2, aligned, d) < 2) continue;
+        const double score = (double)width * groups / ((double)per * most) * (per == 8 ? 0.85 : 1.0) * (groups > 1 ? 1.0 : 0.8);
+        if (score <= best) continue;
+        best = score;
+        b = FwdPlan{per, group, groups};
+    }
+    return b;
+}
+
+template <typename T, int NV, bool ADD>
+int fwd_ring(const NormFwdParams& p, const FwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
+    const int tensors = ADD ? 2 : 1, stages = ring_stages(p.width, b.groups, sizeof(T), tensors, 2, aligned, d);
+    const NormRing r = ring_of(p.width, b.group, b.groups, stages, sizeof(T), tensors, 2, aligned);
+    const long long ctas = (p.rows + b.groups - 1) / b.groups;
+    const unsigned grid = (unsigned)(ctas < d.sms ? ctas : d.sms);
+    if (!aligned) return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, RAGGED>>(p, grid, r, st);
+    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, FULL>>(p, grid, r, st);
+    return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, grid, r, st);
+}
+
 template <typename T, bool ADD>
-void fwd_pick(const NormFwdParams& p, bool aligned, const DevInfo& d, cudaStream_t st) {
+int fwd_pick(NormFwdParams& p, bool aligned, const DevInfo& d, cudaStream_t st) {
     const long long vecs = (p.width + VEC<T> - 1) / VEC<T>;
     // few rows: as many threads a row as it has vectors; many: a warp or less a row while it fits, else eight or four
     // vectors a thread
     const bool few = p.rows < 4 * (long long)d.sms;
+    // Through shared memory: ragged rows (bf16 [5003, 1283] 18.5 -> 16.5 us, with dropout and residual 45 -> 30), and 16-bit rows
+    // behind a residual that would take eight vectors a thread ([32768, 4096] 277 -> 179 us).  The others keep more
+    // threads on an SM without it: [32768, 4096] bf16 97 us against 118, [12608, 768] fp32 with residual 27 against 29.
+    const bool eight = vecs > 192 && (vecs <= 256 || vecs % 256 == 0 || vecs > 2048);
+    if ((!aligned || (ADD && eight && sizeof(T) == 2)) && p.rows >= 16LL * d.sms && p.width > 128) {
+        const FwdPlan b = fwd_plan(p.width, sizeof(T), ADD, aligned, d);
+        if (b.per) {
+            const int e = wait_flag(&p.wait_flag);
+            if (e != MAM_OK) return e;
+            if (b.per == 8) return fwd_ring<T, 8 / VEC<T>, ADD>(p, b, aligned, d, st);
+            if (b.per == 16) return fwd_ring<T, 16 / VEC<T>, ADD>(p, b, aligned, d, st);
+            return fwd_ring<T, 24 / VEC<T>, ADD>(p, b, aligned, d, st);
+        }
+    }
     if (vecs <= 32) {
         fwd_mode<T, 1, ADD>(p, aligned, vecs <= 8 ? 8 : vecs <= 16 ? 16 : 32, 0, st);
     } else if (!few && vecs <= 256) {
@@ -79,6 +171,8 @@ void fwd_pick(const NormFwdParams& p, bool aligned, const DevInfo& d, cudaStream
     } else {
         mam_norm_fwd_wide_kernel<T, ADD, RAGGED><<<(unsigned)p.rows, 1024, 0, st>>>(p);
     }
+    MAM_CUDA(cudaGetLastError());
+    return MAM_OK;
 }
 
 // ---- backward of the norm ----
@@ -88,18 +182,6 @@ struct BwdPlan {
     int group, groups;                     // threads a row, rows at a time in a CTA
     long long parts;                       // partial rows
 };
-
-// A row of the ring in shared memory; ragged ones have up to 15 bytes in front, and are read 16 bytes beyond their end.
-size_t ring_slot(int64_t width, int size, bool aligned) {
-    return aligned ? (size_t)width * size : ((size_t)width * size + 15) / 16 * 16 + 32;
-}
-// shared memory beside the rows: the weight, the barriers, their alignment
-size_t ring_rest(int64_t width) { return (size_t)(width + 8) * 4 + 15 * 4 * 8 + 256; }
-int ring_stages(int64_t width, int groups, int size, int tensors, bool aligned, const DevInfo& d) {
-    const size_t row = tensors * ring_slot(width, size, aligned) * groups, rest = ring_rest(width) + 1024;
-    const long long n = (long long)d.max_smem > (long long)rest ? (long long)((d.max_smem - rest) / row) : 0;
-    return (int)(n < 4 ? n : 4);
-}
 
 // Most partial rows of a backward: a CTA an SM, or the slabs of the wide form.
 long long bwd_parts(int64_t rows, int64_t width, int sms) {
@@ -128,8 +210,8 @@ BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, 
         for (int per : {16, 24, 8}) {
             const int group = threads(per), most = per == 24 ? 384 : per == 8 ? 640 : 512;
             int groups = most / group < 15 ? most / group : 15;      // named barriers
-            while (groups > 1 && ring_stages(width, groups, size, tensors, aligned, d) < 3) --groups;
-            if (groups == 0 || ring_stages(width, groups, size, tensors, aligned, d) < 2) continue;
+            while (groups > 1 && ring_stages(width, groups, size, tensors, 1, aligned, d) < 3) --groups;
+            if (groups == 0 || ring_stages(width, groups, size, tensors, 1, aligned, d) < 2) continue;
             const double score = (double)width * groups / ((double)per * most) * (per == 8 ? 0.85 : 1.0) * (groups > 1 ? 1.0 : 0.8);
             if (score <= best) continue;
             best = score;
@@ -159,42 +241,15 @@ BwdPlan bwd_plan(int64_t rows, int64_t width, int size, bool add, bool aligned, 
     return b;
 }
 
-// Lets a kernel have `bytes` of dynamic shared memory; asked of the runtime once for each device and size that is larger.
-template <auto KERNEL>
-int allow_smem(int bytes) {
-    static std::atomic<int> allowed[64];
-    int dev = 0;
-    MAM_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
-    if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return MAM_OK;
-    MAM_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    allowed[dev].store(bytes, std::memory_order_relaxed);
-    return MAM_OK;
-}
-
-template <auto KERNEL>
-int ring_run(const NormBwdParams& p, const BwdPlan& b, const BwdRing& r, cudaStream_t st) {
-    const int e = allow_smem<KERNEL>((int)r.bytes);
-    if (e != MAM_OK) return e;
-    KERNEL<<<(unsigned)b.parts, b.group * b.groups, r.bytes, st>>>(p, r);
-    MAM_CUDA(cudaGetLastError());
-    return MAM_OK;
-}
 template <typename T, int NV, bool ADD>
 int ring_launch(const NormBwdParams& p, const BwdPlan& b, bool aligned, const DevInfo& d, cudaStream_t st) {
-    BwdRing r{};
-    r.group = b.group;
-    r.groups = b.groups;
-    r.slot_bytes = (unsigned)ring_slot(p.width, sizeof(T), aligned);
-    r.stages = ring_stages(p.width, b.groups, sizeof(T), ADD ? 3 : 2, aligned, d);
-    if (r.stages < 2) return MAM_ERR_UNSUPPORTED;
-    const size_t row = (ADD ? 3 : 2) * (size_t)r.slot_bytes * b.groups;
-    r.weights_at = (unsigned)((row * r.stages + 127) / 128 * 128);
-    r.bars_at = (unsigned)(r.weights_at + (p.width + VEC<T> - 1) / VEC<T> * VEC<T> * 4);
-    r.bytes = r.bars_at + b.groups * r.stages * 8;
-    if (!aligned) return ring_run<mam_norm_bwd_ragged_kernel<T, NV, ADD>>(p, b, r, st);
-    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, FULL>>(p, b, r, st);
-    return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, b, r, st);
+    const int tensors = ADD ? 3 : 2, stages = ring_stages(p.width, b.groups, sizeof(T), tensors, 1, aligned, d);
+    if (stages < 2) return MAM_ERR_UNSUPPORTED;
+    const NormRing r = ring_of(p.width, b.group, b.groups, stages, sizeof(T), tensors, 1, aligned);
+    const unsigned ctas = (unsigned)b.parts;
+    if (!aligned) return ring_run<mam_norm_bwd_ragged_kernel<T, NV, ADD>>(p, ctas, r, st);
+    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, FULL>>(p, ctas, r, st);
+    return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, ctas, r, st);
 }
 
 template <typename T, bool ADD, int MODE>
@@ -332,7 +387,7 @@ int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int
         return MAM_ERR_INVALID_ARGUMENT;
     if (rows > MOST_ROWS || width > MOST_WIDTH) return MAM_ERR_UNSUPPORTED;
     NormFwdParams p{x, residual, weight, bias, y, sum, reinterpret_cast<float2*>(stats), rows, width, x_pitch,
-                    residual_pitch, eps, 1.0f / (float)width, param_dtype == MAM_F32, {}};
+                    residual_pitch, eps, 1.0f / (float)width, param_dtype == MAM_F32, nullptr, {}};
     int st = drop_args(drop_rate, drop_seed, drop_seed_at, &p.drop);
     if (st != MAM_OK) return st;
     const DevInfo* d = nullptr;
@@ -343,13 +398,11 @@ int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int
                      aligned16(residual) && aligned16(y) && aligned16(sum) && aligned16(weight) && aligned16(bias);
     cudaStream_t cs = (cudaStream_t)stream;
     switch (dtype) {
-        case MAM_F32: residual ? fwd_pick<float, true>(p, vec, *d, cs) : fwd_pick<float, false>(p, vec, *d, cs); break;
-        case MAM_F16: residual ? fwd_pick<__half, true>(p, vec, *d, cs) : fwd_pick<__half, false>(p, vec, *d, cs); break;
+        case MAM_F32: return residual ? fwd_pick<float, true>(p, vec, *d, cs) : fwd_pick<float, false>(p, vec, *d, cs);
+        case MAM_F16: return residual ? fwd_pick<__half, true>(p, vec, *d, cs) : fwd_pick<__half, false>(p, vec, *d, cs);
         default:
-            residual ? fwd_pick<__nv_bfloat16, true>(p, vec, *d, cs) : fwd_pick<__nv_bfloat16, false>(p, vec, *d, cs);
+            return residual ? fwd_pick<__nv_bfloat16, true>(p, vec, *d, cs) : fwd_pick<__nv_bfloat16, false>(p, vec, *d, cs);
     }
-    MAM_CUDA(cudaGetLastError());
-    return MAM_OK;
 }
 
 size_t mam_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width) {

@@ -4,8 +4,9 @@
 //   h = (s - mu) r                                                y = h w + b
 //   a = gy w    ds = r (a - mean(a) - h mean(a h)) + gs           dx = drop(ds)     dw = sum_rows gy h    db = sum_rows gy
 //
-// The norm reads the sum as it is stored, rounded: the fused call then equals the residual addition followed by the norm
-// bit for bit, and the backward, which has only the stored sum, differentiates exactly what the forward computed.
+// The norm reads the sum as it is stored, rounded: the fused call then equals the residual addition followed by the norm (s bit
+// for bit, y up to the order of a row's sums), and the backward, which has only the stored sum, differentiates exactly what
+// the forward computed.
 //
 // Bound by memory: forward one read and one write of the rows (two and two with the residual), backward two reads and one
 // write (three and two).  A row stays in registers between its load and its store; statistics take two reductions, the
@@ -16,6 +17,10 @@
 #include "mam_vec.cuh"
 
 namespace mamb200 {
+
+// threads of a CTA that an SM's registers hold, by the values each keeps in the forward's ring
+template <int PER>
+constexpr int FWD_RING_THREADS = PER == 8 ? 1024 : PER == 16 ? 768 : 640;
 
 struct NormFwdParams {
     const void* x;
@@ -28,6 +33,7 @@ struct NormFwdParams {
     long long rows, width, x_pitch, res_pitch;
     float eps, inv_width;
     bool params_f32;
+    int* wait_flag;            // set where a bounded wait ran out
     DropArgs drop;
 };
 
@@ -119,6 +125,10 @@ __device__ __forceinline__ float2 row_stats(float mu, float d1, float d2, float 
 }
 
 // Rows of up to NV vectors a thread, held in registers.  CTA: a CTA a row; else LANES lanes a row, 128 / LANES rows a CTA.
+// Loads of a whole row at once and as many threads on an SM as the registers allow keep the memory busy: 85 % of the copy rate at
+// [32768, 4096] bf16 (97 us; four vectors a thread instead of eight 108, for the reductions' instructions are paid per
+// thread), 94 % at [4096, 8192] fp32.  FULL leaves out the tests for columns: 28 -> 14 instructions an element with the packed
+// pairs.
 template <typename T, int NV, bool ADD, int MODE, bool CTA, int LANES>
 __global__ void __launch_bounds__(!CTA ? 128 : NV <= 2 ? 1024 : 512)
 mam_norm_fwd_kernel(const __grid_constant__ NormFwdParams p) {
@@ -199,6 +209,185 @@ mam_norm_fwd_kernel(const __grid_constant__ NormFwdParams p) {
             q = pack<T>(w);
         }
         store_vec<T, MODE>(static_cast<T*>(p.y) + row * p.width + col(i), q, width - col(i), t, nt, i == 0, i == NV - 1, carry);
+    }
+}
+
+// Places in shared memory of a ring of rows: `stages` rows of each of `groups` groups of `group` threads (whole warps) are
+// there or on their way by bulk copies, so that loads go on whatever the registers leave room for.
+struct NormRing {
+    int group, groups, stages;
+    unsigned slot_bytes;                   // of one tensor's row
+    unsigned weights_at, bars_at, bytes;   // the parameters, the barriers; the whole
+};
+
+// Many rows that are ragged, or too wide for the next kernel's loads to be held: one CTA an SM walks them with the parameters
+// in shared memory, in fp32.  A group's row leaves its stage for the
+// registers before the first reduction; behind that barrier thread 0 sends for the row `stages` ahead.  RAGGED rows are
+// copied with the aligned 16 bytes at either end, which belong to the rows beside them; the first and the last row have no
+// such neighbours and are brought element by element.
+template <typename T, int NV, bool ADD, int MODE>
+__global__ void __launch_bounds__(FWD_RING_THREADS<NV * VEC<T>>)
+mam_norm_fwd_ring_kernel(const __grid_constant__ NormFwdParams p, const __grid_constant__ NormRing ring) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float2 slot[2][32];
+    constexpr int V = VEC<T>, HALVES = V / 4, TENSORS = ADD ? 2 : 1, MOST = 32;
+    const int group = ring.group, groups = ring.groups, g = threadIdx.x / group, t = threadIdx.x - g * group;
+    const int lane = threadIdx.x & 31, warps = group >> 5, slot0 = (g * group) >> 5;
+    const int width = (int)p.width;
+    const int vec0 = (t >> 5) * NV * 32 + lane;     // a warp's vectors follow one another
+    auto col = [&](int i) { return (vec0 + i * 32) * V; };
+    auto count = [&](int i) { return MODE == FULL ? V : min(V, width - col(i)); };
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + ring.bars_at) + g * ring.stages;
+    unsigned char* mine = smem + (size_t)g * ring.stages * TENSORS * ring.slot_bytes;      // [stage][x, residual][row]
+    // weight and bias, the halves of a vector of eight apart: a warp's 16-byte reads then meet no bank twice
+    float4* params = reinterpret_cast<float4*>(smem + ring.weights_at);
+    const int vecs = (width + V - 1) / V;
+    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+        float2 w[V / 2], b[V / 2];
+        load_param<T, MODE>(p.weight, p.params_f32, v * V, min(V, width - v * V), 1.f, w);
+        load_param<T, MODE>(p.bias, p.params_f32, v * V, min(V, width - v * V), 0.f, b);
+#pragma unroll
+        for (int k = 0; k < HALVES; ++k) {
+            params[k * vecs + v] = make_float4(w[2 * k].x, w[2 * k].y, w[2 * k + 1].x, w[2 * k + 1].y);
+            params[(HALVES + k) * vecs + v] = make_float4(b[2 * k].x, b[2 * k].y, b[2 * k + 1].x, b[2 * k + 1].y);
+        }
+    }
+    if (t == 0) {
+        for (int k = 0; k < ring.stages; ++k) mbar_init(full + k, 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+
+    const long long step = (long long)gridDim.x * groups;
+    const T *x0 = static_cast<const T*>(p.x), *r0 = static_cast<const T*>(p.residual);
+    const unsigned row_bytes = (unsigned)width * sizeof(T);
+    auto misfit = [](const T* q) { return MODE == RAGGED ? (unsigned)(reinterpret_cast<uintptr_t>(q) & 15u) : 0u; };
+    auto edge = [&](long long row) { return MODE == RAGGED && (row == 0 || row == p.rows - 1); };
+    auto send = [&](long long row, int stage) {
+        if (row >= p.rows) return;
+        if (edge(row)) {
+            mbar_arrive(full + stage);
+            return;
+        }
+        unsigned char* to = mine + (size_t)stage * TENSORS * ring.slot_bytes;
+        const T *px = x0 + row * p.x_pitch, *pr = r0 + row * p.res_pitch;
+        const unsigned bx = MODE == RAGGED ? (misfit(px) + row_bytes + 15u) & ~15u : row_bytes;
+        const unsigned br = !ADD ? 0u : MODE == RAGGED ? (misfit(pr) + row_bytes + 15u) & ~15u : row_bytes;
+        mbar_expect_tx(full + stage, bx + br);
+        bulk_load(to, reinterpret_cast<const unsigned char*>(px) - misfit(px), bx, full + stage);
+        if (ADD) bulk_load(to + ring.slot_bytes, reinterpret_cast<const unsigned char*>(pr) - misfit(pr), br, full + stage);
+    };
+    long long row = (long long)blockIdx.x * groups + g;
+    if (t == 0)
+        for (int k = 0; k < ring.stages; ++k) send(row + k * step, k);
+    auto meet = [&]() {
+        if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
+        else __syncwarp();
+    };
+    long long at = row * p.width;
+    const long long at_step = step * p.width;
+    const unsigned long long seed = ADD && p.drop.on ? p.drop.seed_now() : 0;
+    const unsigned long long drop_step = (unsigned long long)(at_step >> 1) * MAM_DROP_STEP;
+    unsigned long long start = mam_drop_start(seed, at + vec0 * V);
+    uint4 carry = make_uint4(0u, 0u, 0u, 0u);
+    int stage = 0;
+    unsigned phase = 0;
+    bool lost = false;
+    for (; row < p.rows; row += step, at += at_step, start += drop_step) {
+        unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
+        if (!mbar_wait_bounded(full + stage, phase, lost ? 1024 : 1u << 22)) {
+            lost = true;            // the results are void, but every barrier is still met and every copy waited for
+            *p.wait_flag = 1;
+        }
+        unsigned skip_x = 0, skip_r = 0;
+        if constexpr (MODE == RAGGED) {
+            const T *px = x0 + row * p.x_pitch, *pr = r0 + row * p.res_pitch;
+            skip_x = misfit(px);
+            skip_r = misfit(pr);
+            if (edge(row)) {
+                T *dx = reinterpret_cast<T*>(from + skip_x), *dr = reinterpret_cast<T*>(from + ring.slot_bytes + skip_r);
+                for (int c = t; c < width; c += group) {
+                    dx[c] = px[c];
+                    if (ADD) dr[c] = pr[c];
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // before a later copy into this stage
+                meet();
+            }
+            start = mam_drop_start(seed, at + vec0 * V);
+        }
+        const bool odd = MODE == RAGGED && ((at + vec0 * V) & 1);
+        float2 v[NV][V / 2], s = splat2(0.f), d1 = s, d2 = s;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint4* q = reinterpret_cast<const uint4*>(from) + vec0 + i * 32;
+            uint4 qx = make_uint4(0u, 0u, 0u, 0u);
+            if (count(i) > 0) {
+                if constexpr (MODE == RAGGED) qx = cut<T>(q[0], q[1], skip_x);
+                else qx = *q;
+                if constexpr (ADD) {
+                    const uint4* k = reinterpret_cast<const uint4*>(from + ring.slot_bytes) + vec0 + i * 32;
+                    uint4 qr;
+                    if constexpr (MODE == RAGGED) qr = cut<T>(k[0], k[1], skip_r);
+                    else qr = *k;
+                    qx = add_residual<T>(qx, qr, p.drop, start + (unsigned long long)(i * 32 * (V / 2)) * MAM_DROP_STEP, odd);
+                }
+                unpack<T>(qx, v[i]);
+                if (MODE == RAGGED && count(i) < V) keep_first<T>(v[i], count(i));
+                s = add2(s, total<T>(v[i]));
+            }
+            if constexpr (ADD)
+                store_vec<T, MODE>(static_cast<T*>(p.sum) + at + col(i), qx, MODE == FULL ? V : width - col(i), lane, 32, i == 0,
+                                   i == NV - 1, carry);
+        }
+        float mu = lane_sum<32>(sum2(s));
+        if (warps > 1 && lane == 0) slot[0][threadIdx.x >> 5].x = mu;
+        meet();
+        // all have this row in their registers
+        if (t == 0) send(row + ring.stages * step, stage);
+        if (warps > 1) mu = lane_sum<MOST>(lane < warps ? slot[0][slot0 + lane].x : 0.f);
+        mu *= p.inv_width;
+        const float2 minus = splat2(-mu);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (count(i) > 0) {
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) v[i][j] = add2(v[i][j], minus);
+                if (MODE == RAGGED && count(i) < V) keep_first<T>(v[i], count(i));
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) d2 = fma2(v[i][j], v[i][j], d2);
+                d1 = add2(d1, total<T>(v[i]));
+            }
+        float2 d = lane_sum2<32>(sum2(d1), sum2(d2));
+        if (warps > 1) {
+            if (lane == 0) slot[1][threadIdx.x >> 5] = d;
+            meet();
+            d = lane < warps ? slot[1][slot0 + lane] : make_float2(0.f, 0.f);
+            d = lane_sum2<MOST>(d.x, d.y);
+        }
+        float off;
+        const float2 st = row_stats(mu, d.x, d.y, p.inv_width, p.eps, off);
+        if (p.stats && t == 0) p.stats[row] = st;
+        const float2 r2 = splat2(st.y), o2 = splat2(-off);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if (count(i) > 0) {
+                Vals<T> y;
+#pragma unroll
+                for (int k = 0; k < HALVES; ++k) {
+                    const float4 w = params[k * vecs + vec0 + i * 32], b = params[(HALVES + k) * vecs + vec0 + i * 32];
+                    y[2 * k] = fma2(mul2(add2(v[i][2 * k], o2), r2), make_float2(w.x, w.y), make_float2(b.x, b.y));
+                    y[2 * k + 1] = fma2(mul2(add2(v[i][2 * k + 1], o2), r2), make_float2(w.z, w.w), make_float2(b.z, b.w));
+                }
+                q = pack<T>(y);
+            }
+            store_vec<T, MODE>(static_cast<T*>(p.y) + at + col(i), q, MODE == FULL ? V : width - col(i), lane, 32, i == 0,
+                               i == NV - 1, carry);
+        }
+        if (++stage == ring.stages) {
+            stage = 0;
+            phase ^= 1;
+        }
     }
 }
 
@@ -440,15 +629,9 @@ __global__ void __launch_bounds__(512) mam_norm_bwd_narrow_kernel(const __grid_c
 // vectors in registers instead, bf16 [32768, 4096] took 155 us (this: 130) and with dropout 336 (211).
 // A row's stage is free when its group has passed the next row's barrier; thread 0 of the group then sends for the row
 // `stages - 1` ahead.
-struct BwdRing {
-    int group, groups, stages;
-    unsigned slot_bytes;                   // of one tensor's row
-    unsigned weights_at, bars_at, bytes;   // places in shared memory, and its size
-};
-
 template <typename T, int NV, bool ADD, int MODE>
 __global__ void __launch_bounds__(NV * VEC<T> == 8 ? 640 : NV * VEC<T> == 24 ? 384 : 512)
-mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_constant__ BwdRing ring) {
+mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_constant__ NormRing ring) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float2 slot[2][32];
     constexpr int V = VEC<T>, HALVES = V / 4, TENSORS = ADD ? 3 : 2, MOST = NV * V == 8 ? 32 : 16;      // warps a group can have
@@ -619,7 +802,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
 // template the aligned form lost 3 to 8 %.)  bf16 [5003, 1283] 25 us, with the next row's vectors in registers instead 40.
 template <typename T, int NV, bool ADD>
 __global__ void __launch_bounds__(NV * VEC<T> == 8 ? 640 : NV * VEC<T> == 24 ? 384 : 512)
-mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid_constant__ BwdRing ring) {
+mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid_constant__ NormRing ring) {
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float2 slot[2][32];
     constexpr int V = VEC<T>, HALVES = V / 4, TENSORS = ADD ? 3 : 2, MOST = NV * V == 8 ? 32 : 16;      // warps a group can have

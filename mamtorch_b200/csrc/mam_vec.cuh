@@ -162,10 +162,7 @@ struct RowSrc {
         if constexpr (MODE != RAGGED && !STREAM) {
             return *reinterpret_cast<const uint4*>(p);
         } else if constexpr (MODE != RAGGED) {
-            uint4 q;
-            asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
-            return q;
+            return __ldcg(reinterpret_cast<const uint4*>(p));
         } else {
             const uintptr_t a = reinterpret_cast<uintptr_t>(p) - off;
             if (inside || (a >= lo && a + 32 <= hi))

@@ -460,8 +460,8 @@ def layer_norm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = No
 def dropout_add_layer_norm(x: Tensor, residual: Tensor, weight: Tensor | None = None, bias: Tensor | None = None,
                            eps: float = 1e-5, drop_rate: float = 0.0, drop_seed=None):
     """(y, s): s = residual + dropout(x), the residual stream behind a block, and y = layer_norm(s), the input of the next.
-    One pass forward and one backward; equal to `dropout(x, ..., residual)` followed by `layer_norm` bit for bit (the
-    norm reads s as it is stored)."""
+    One pass forward and one backward; equal to `dropout(x, ..., residual)` followed by `layer_norm`, which reads s as it
+    is stored: s bit for bit, y up to the order of a row's fp32 sums."""
     f = _C.dropout_add_layer_norm if _eager(x) else _ops.dropout_add_layer_norm.default
     return f(x, residual, weight, bias, eps, *_drop_args(drop_rate, drop_seed))
 
