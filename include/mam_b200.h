@@ -393,8 +393,9 @@ int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int
 
 /* Its backward, from s (x or sum, rows s_pitch apart) and stats.  gy: gradient of y; gsum: gradient of sum; either may be
  * NULL (zeros).  ds: gradient of s, which is the residual's too.  dx, required where drop_rate > 0: drop(ds), the gradient
- * of x; else NULL, and ds is the gradient of x.  dweight and dbias, each optional, in param_dtype: summed in a fixed order;
- * with either of them the call needs the workspace (256-byte aligned). */
+ * of x; else optional, and equal to ds.  dweight and dbias, each optional, in param_dtype: summed in a fixed order;
+ * with either of them the call needs the workspace (256-byte aligned).  Rows travel through shared memory under bounded
+ * waits (mam_check_device_flag), in the forward for some shapes too. */
 size_t mam_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
 int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t s_pitch, const float* stats,
                        const void* weight, int param_dtype,

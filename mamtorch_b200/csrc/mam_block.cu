@@ -19,6 +19,7 @@ bool natural(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) 
 
 int drop_args(float rate, uint64_t seed, const int64_t* seed_at, DropArgs* d) {
     *d = DropArgs{};
+    d->scale = 1.f;      // nothing dropped leaves the values as they are
     unsigned thr = 0;
     if (!drop_threshold(rate, &thr) || (reinterpret_cast<uintptr_t>(seed_at) & 7u)) return MAM_ERR_INVALID_ARGUMENT;
     if (rate == 0.f) return MAM_OK;
@@ -43,22 +44,23 @@ int ring_stages(int64_t width, int groups, int size, int tensors, int params, bo
     return (int)(n < 4 ? n : 4);
 }
 
-// Lets a kernel have `bytes` of dynamic shared memory; asked of the runtime once for each device and size that is larger.
+// Lets a kernel have all the dynamic shared memory that ring_stages counts with: asked of the runtime once for each device,
+// and always the same, so that calls from several threads cannot take it from one another.
 template <auto KERNEL>
-int allow_smem(int bytes) {
-    static std::atomic<int> allowed[64];
+int allow_smem(const DevInfo& d) {
+    static std::atomic<bool> allowed[64];
     int dev = 0;
     MAM_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
-    if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return MAM_OK;
-    MAM_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    allowed[dev].store(bytes, std::memory_order_relaxed);
+    if (allowed[dev].load(std::memory_order_acquire)) return MAM_OK;
+    MAM_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, d.max_smem - 1024));
+    allowed[dev].store(true, std::memory_order_release);
     return MAM_OK;
 }
 
 template <auto KERNEL, class Params>
-int ring_run(const Params& p, unsigned ctas, const NormRing& r, cudaStream_t st) {
-    const int e = allow_smem<KERNEL>((int)r.bytes);
+int ring_run(const Params& p, unsigned ctas, const NormRing& r, const DevInfo& d, cudaStream_t st) {
+    const int e = allow_smem<KERNEL>(d);
     if (e != MAM_OK) return e;
     KERNEL<<<ctas, r.group * r.groups, r.bytes, st>>>(p, r);
     MAM_CUDA(cudaGetLastError());
@@ -75,6 +77,7 @@ NormRing ring_of(int64_t width, int group, int groups, int stages, int size, int
     r.bytes = r.bars_at + groups * stages * 8;
     return r;
 }
+
 // ---- forward of the norm ----
 template <typename T, int NV, bool ADD, int MODE>
 void fwd_launch(const NormFwdParams& p, int lanes, int threads, cudaStream_t st) {
@@ -126,9 +129,9 @@ int fwd_ring(const NormFwdParams& p, const FwdPlan& b, bool aligned, const DevIn
     const NormRing r = ring_of(p.width, b.group, b.groups, stages, sizeof(T), tensors, 2, aligned);
     const long long ctas = (p.rows + b.groups - 1) / b.groups;
     const unsigned grid = (unsigned)(ctas < d.sms ? ctas : d.sms);
-    if (!aligned) return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, RAGGED>>(p, grid, r, st);
-    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, FULL>>(p, grid, r, st);
-    return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, grid, r, st);
+    if (!aligned) return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, RAGGED>>(p, grid, r, d, st);
+    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, FULL>>(p, grid, r, d, st);
+    return ring_run<mam_norm_fwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, grid, r, d, st);
 }
 
 template <typename T, bool ADD>
@@ -247,9 +250,9 @@ int ring_launch(const NormBwdParams& p, const BwdPlan& b, bool aligned, const De
     if (stages < 2) return MAM_ERR_UNSUPPORTED;
     const NormRing r = ring_of(p.width, b.group, b.groups, stages, sizeof(T), tensors, 1, aligned);
     const unsigned ctas = (unsigned)b.parts;
-    if (!aligned) return ring_run<mam_norm_bwd_ragged_kernel<T, NV, ADD>>(p, ctas, r, st);
-    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, FULL>>(p, ctas, r, st);
-    return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, ctas, r, st);
+    if (!aligned) return ring_run<mam_norm_bwd_ragged_kernel<T, NV, ADD>>(p, ctas, r, d, st);
+    if (p.width == (long long)b.group * NV * VEC<T>) return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, FULL>>(p, ctas, r, d, st);
+    return ring_run<mam_norm_bwd_ring_kernel<T, NV, ADD, ALIGNED>>(p, ctas, r, d, st);
 }
 
 template <typename T, bool ADD, int MODE>

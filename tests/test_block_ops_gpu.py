@@ -716,10 +716,14 @@ def test_c_abi_without_torch_operators(cuda):
     check(dx, drop64(dv, 0.1, 7), torch.float32, 2 * scale, "dx")
     assert L.mam_layer_norm_bwd(*args, None, 0, st) == 3 and L.mam_layer_norm_bwd(*args, p(ws), nbytes - 1, st) == 3
     assert L.mam_layer_norm_bwd(*args, ctypes.c_void_p(ws.data_ptr() + 4), nbytes, st) == 3
+    # a second gradient although nothing is dropped: the same
+    none = (0.0, 7, None)
+    assert L.mam_layer_norm_bwd(*args[:7], *none, p(ds), p(dx), p(dw), p(db), rows, width, 0, p(ws), nbytes, st) == 0
+    assert torch.equal(ds, dx)
     # without the parameters' gradients no workspace is needed
     ds2 = torch.empty_like(ds)
     assert L.mam_layer_norm_bwd(*args[:10], p(ds2), p(dx), None, None, rows, width, 0, None, 0, st) == 0
-    assert torch.equal(ds, ds2)
+    assert torch.equal(ds, ds2) and not torch.equal(ds, dx)
     assert L.mam_check_device_flag() == 0
 
 
