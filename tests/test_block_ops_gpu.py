@@ -621,6 +621,31 @@ def test_on_a_stream_of_its_own_and_two_at_once(cuda):
             assert all(torch.equal(p, q) for p, q in zip(run, ref))
 
 
+def test_from_several_threads_at_once(cuda):
+    """First calls of kernels with different amounts of shared memory, from threads of their own."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from mamtorch_b200.nn import functional as MF
+
+    def work(k):
+        width = (200, 1000, 2500, 4500, 7000, 8192)[k % 6]
+        t = DTYPES[k % 3]
+        x, r, g = (inputs((300, width), t, 10 * k + j, cuda) for j in range(3))
+        x.requires_grad_()
+        w, b = (p.requires_grad_() for p in params(width, t, k, cuda))
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+            y, s = MF.dropout_add_layer_norm(MF.gelu(x, 0.1, k), r, w, b, 1e-5, 0.1, k)
+            out = [y, s, *torch.autograd.grad((y, s), (x, w, b), (g, g))]
+            torch.cuda.current_stream().synchronize()
+        return out
+
+    with ThreadPoolExecutor(6) as pool:
+        at_once = list(pool.map(work, range(18)))
+    for k, out in enumerate(at_once):
+        assert all(torch.equal(p, q) for p, q in zip(out, work(k)))
+
+
 def test_captured_steps_replay_with_new_seeds(cuda):
     from mamtorch_b200.nn import functional as MF
 
