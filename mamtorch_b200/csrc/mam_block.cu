@@ -318,36 +318,25 @@ int bwd_type(const NormBwdParams& p, const BwdPlan& b, bool vec, bool add, void*
 }
 
 // ---- pointwise ----
-constexpr long long POINT_SPLIT = 1 << 18;   // elements from which a second launch costs less than ragged loads and stores
 template <typename T, int NV, int OP>
-int point_run(const PointParams& p, bool whole, cudaStream_t st) {
-    const long long per = (long long)POINT_THREADS * VEC<T> * NV, blocks = (p.n + per - 1) / per;
+int point_run(PointParams p, bool aligned, cudaStream_t st) {
+    const long long per = (long long)POINT_THREADS * VEC<T> * NV;
+    const int tail = aligned ? (int)(p.n % VEC<T>) : 0;
+    p.n -= tail;
+    p.tail = tail;
+    const long long blocks = (p.n + per - 1) / per + (tail ? 1 : 0);
     if (blocks > 2147483647LL) return MAM_ERR_UNSUPPORTED;
-    if (whole) mam_point_kernel<T, NV, OP, ALIGNED><<<(unsigned)blocks, POINT_THREADS, 0, st>>>(p);
-    else mam_point_kernel<T, NV, OP, RAGGED><<<(unsigned)blocks, POINT_THREADS, 0, st>>>(p);
+    if (tail) mam_point_kernel<T, NV, OP, ALIGNED, true><<<(unsigned)blocks, POINT_THREADS, 0, st>>>(p);
+    else if (aligned) mam_point_kernel<T, NV, OP, ALIGNED, false><<<(unsigned)blocks, POINT_THREADS, 0, st>>>(p);
+    else mam_point_kernel<T, NV, OP, RAGGED, false><<<(unsigned)blocks, POINT_THREADS, 0, st>>>(p);
     MAM_CUDA(cudaGetLastError());
     return MAM_OK;
 }
 template <typename T, int OP>
 int point_launch(const PointParams& p, bool aligned, const DevInfo& d, cudaStream_t st) {
-    const long long tail = p.n % VEC<T>;
-    if (aligned && tail && p.n > POINT_SPLIT) {
-        // whole vectors, and a second launch for the rest
-        PointParams q = p;
-        q.n = p.n - tail;
-        int e = point_launch<T, OP>(q, true, d, st);
-        if (e != MAM_OK) return e;
-        const long long whole = q.n;
-        q.x = static_cast<const T*>(p.x) + whole;
-        q.other = p.other ? static_cast<const T*>(p.other) + whole : nullptr;
-        q.out = static_cast<T*>(p.out) + whole;
-        q.first = p.first + whole;
-        q.n = tail;
-        return point_run<T, 1, OP>(q, false, st);
-    }
     // four vectors a thread, or one where that leaves SMs without work
-    if (p.n > 4LL * POINT_THREADS * VEC<T> * 2 * d.sms) return point_run<T, 4, OP>(p, aligned && !tail, st);
-    return point_run<T, 1, OP>(p, aligned && !tail, st);
+    if (p.n > 4LL * POINT_THREADS * VEC<T> * 2 * d.sms) return point_run<T, 4, OP>(p, aligned, st);
+    return point_run<T, 1, OP>(p, aligned, st);
 }
 template <int OP>
 int point(const void* x, const void* other, void* out, int64_t n, int dtype, float rate, uint64_t seed,

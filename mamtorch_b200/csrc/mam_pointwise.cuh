@@ -15,7 +15,7 @@ struct PointParams {
     const void* other;     // residual (or nullptr), or the upstream gradient
     void* out;
     long long n;
-    long long first;       // the place of x[0] in the tensor, even: where its draws begin
+    int tail;              // elements behind the n of the whole vectors (TAIL)
     DropArgs drop;
 };
 
@@ -86,9 +86,11 @@ __device__ __forceinline__ void point_apply(float2 (&x)[N], const float2 (&o)[N]
 constexpr int POINT_THREADS = 128;
 
 // NV vectors a thread, all loads first; a CTA a block (CTAs that walk over several blocks took a sixth fewer instructions and
-// a tenth longer: their loads wait for the stores before them).  ALIGNED: whole vectors only, n is a multiple of them.
+// a tenth longer: their loads wait for the stores before them).  ALIGNED: whole vectors only, n is a multiple of them; with TAIL
+// one thread of a last CTA does the elements behind them, pair by pair (an instance of its own: the loop's registers cost the
+// others a tenth).
 // RAGGED: any n and any alignment, with the loads and stores of ragged rows, the whole tensor being one row.
-template <typename T, int NV, int OP, int MODE>
+template <typename T, int NV, int OP, int MODE, bool TAIL>
 __global__ void __launch_bounds__(POINT_THREADS, 8) mam_point_kernel(const __grid_constant__ PointParams p) {
     constexpr int V = VEC<T>;
     const bool has = p.other != nullptr;
@@ -100,7 +102,24 @@ __global__ void __launch_bounds__(POINT_THREADS, 8) mam_point_kernel(const __gri
     const long long base = MODE == RAGGED
         ? (((long long)blockIdx.x * (POINT_THREADS / 32) + (threadIdx.x >> 5)) * (NV * 32) + (threadIdx.x & 31)) * V
         : ((long long)blockIdx.x * NV * POINT_THREADS + threadIdx.x) * V;
-    const unsigned long long start = p.drop.on ? mam_drop_start(p.drop.seed_now(), p.first + base) : 0;
+    if constexpr (TAIL) {
+        if (blockIdx.x == gridDim.x - 1) {
+            if (threadIdx.x > 0) return;
+            const unsigned long long seed = p.drop.on ? p.drop.seed_now() : 0;
+            const T *xt = static_cast<const T*>(p.x) + p.n, *ot = static_cast<const T*>(p.other) + p.n;
+#pragma unroll 1
+            for (int e = 0; e < p.tail; e += 2) {
+                const bool two = e + 1 < p.tail;
+                float2 f[1] = {make_float2(to_f32(xt[e]), two ? to_f32(xt[e + 1]) : 0.f)}, g[1] = {splat2(0.f)};
+                if (has) g[0] = make_float2(to_f32(ot[e]), two ? to_f32(ot[e + 1]) : 0.f);
+                point_apply<OP>(f, g, has, p.drop, mam_drop_start(seed, p.n + e));
+                out[p.n + e] = from_f32<T>(f[0].x);
+                if (two) out[p.n + e + 1] = from_f32<T>(f[0].y);
+            }
+            return;
+        }
+    }
+    const unsigned long long start = p.drop.on ? mam_drop_start(p.drop.seed_now(), base) : 0;
     uint4 px[NV], po[NV], carry = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
