@@ -3,7 +3,7 @@
 // The `*_forward` / `*_backward` operators validate, allocate and call the library (CUDA only: a CPU tensor gets the
 // dispatcher's NotImplementedError).  The differentiable ones (layer_norm, dropout_add_layer_norm, dropout, gelu) call
 // them below an autograd node where a gradient is wanted, and directly where none is: for a few rows the host's time
-// is the call's time.
+// is the call's time.  Each differentiates once and in reverse; what would be anything else is refused, never a zero.
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -236,16 +236,47 @@ bool wants_grad(const Ts&... ts) {
 }
 Tensor plain(const OptTensor& t) { return has(t) ? *t : Tensor(); }
 
-// Gradients are not differentiable again: under create_graph they carry a node that says so when it is run.
-variable_list once(variable_list&& grads, bool graph) {
-    if (graph)
-        for (auto& g : grads)
-            if (g.defined())
-                g = (*std::make_shared<torch::autograd::DelayedError>(
-                    "mamtorch_b200: layer_norm, dropout and gelu are differentiable once", 1))(
-                    {g.detach().requires_grad_(true)})[0];
-    return std::move(grads);
+// A tangent would be lost below the autograd keys, and torch takes a missing one for zero.
+template <class... Ts>
+void refuse_tangents(const Ts&... ts) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!((ts.defined() && ts._fw_grad(0).defined()) || ...),
+                                "mamtorch_b200: layer_norm, dropout and gelu have no forward-mode derivative");
 }
+
+// Whether a transform of torch.func is around the call: then every operator goes through the dispatcher, which takes it to
+// the transform's levels one by one.
+bool transformed() { return c10::impl::tls_is_dispatch_key_included(at::DispatchKey::FuncTorchDynamicLayerFrontMode); }
+
+// The inner operators carry no derivative: where one would be wanted their outputs get a node that says so when it is run.
+// A gradient that is differentiated again (create_graph, nested transforms) ends there.
+const Tensor& tensor_of(const Tensor& t) { return t; }
+Tensor tensor_of(const OptTensor& t) { return plain(t); }
+template <class T>
+Tensor tensor_of(const T&) { return Tensor(); }
+void dead_end(Tensor& t, const std::shared_ptr<torch::autograd::Error>& node) { torch::autograd::set_history(t, node); }
+void dead_end(std::vector<Tensor>& ts, const std::shared_ptr<torch::autograd::Error>& node) {
+    for (auto& t : ts) dead_end(t, node);
+}
+template <class Fn, const char* NAME>
+struct Inner;
+template <class R, class... A, const char* NAME>
+struct Inner<R(A...), NAME> {
+    static R call(A... args) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<R(A...)>();
+        refuse_tangents(tensor_of(args)...);
+        std::shared_ptr<torch::autograd::Error> node;
+        if (wants_grad(tensor_of(args)...))
+            node.reset(new torch::autograd::Error("mamtorch_b200: layer_norm, dropout and gelu are differentiable once",
+                                                  torch::autograd::collect_next_edges(tensor_of(args)...)),
+                       torch::autograd::deleteNode);
+        R out = [&] {
+            at::AutoDispatchBelowADInplaceOrView below;
+            return op.call(args...);
+        }();
+        if (node) dead_end(out, node);
+        return out;
+    }
+};
 
 // The nodes are written out, as torch's own are: the generic C++ Function keeps its arguments in a dictionary by name, which
 // took as long as an allocation.
@@ -276,8 +307,6 @@ struct NormBackward : BlockNode {       // inputs: x, residual, weight, bias
         weight.reset_data();
     }
     variable_list apply(variable_list&& g) override {
-        const bool graph = at::GradMode::is_enabled();
-        at::AutoGradMode off(false);
         const Tensor gs = add ? g[1] : Tensor();
         variable_list r(4);
         if (!g[0].defined() && !gs.defined()) return r;
@@ -297,15 +326,13 @@ struct NormBackward : BlockNode {       // inputs: x, residual, weight, bias
         }
         if (want_w) r[2] = std::move(d[next++]);
         if (want_b) r[3] = std::move(d[next]);
-        return once(std::move(r), graph);
+        return r;
     }
 };
 
 struct DropoutBackward : BlockNode {    // inputs: x, residual
     std::string name() const override { return "MamDropoutBackward"; }
     variable_list apply(variable_list&& g) override {
-        const bool graph = at::GradMode::is_enabled();
-        at::AutoGradMode off(false);
         variable_list r(2);
         if (!g[0].defined()) return r;
         if (task_should_compute_output(0)) {
@@ -313,7 +340,7 @@ struct DropoutBackward : BlockNode {    // inputs: x, residual
             r[0] = rate > 0 ? op.call(g[0], std::nullopt, rate, seed, opt(seed_at.unpack())) : g[0];
         }
         if (task_should_compute_output(1)) r[1] = g[0];
-        return once(std::move(r), graph);
+        return r;
     }
 };
 
@@ -325,27 +352,25 @@ struct GeluBackward : BlockNode {       // input: x
         x.reset_data();
     }
     variable_list apply(variable_list&& g) override {
-        const bool graph = at::GradMode::is_enabled();
-        at::AutoGradMode off(false);
         variable_list r(1);
         if (!g[0].defined()) return r;
         MAM_OP(op, gelu_backward);
         r[0] = op.call(g[0], x.unpack(), rate, seed, opt(seed_at.unpack()));
-        return once(std::move(r), graph);
+        return r;
     }
 };
 
-// y, s with a residual
-std::vector<Tensor> norm(const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias,
-                         double eps, double rate, int64_t seed, const OptTensor& seed_at) {
+// The differentiable operators.  Without a transform they call the inner operator themselves; with one, their own operator
+// below the autograd keys, so that the levels further out differentiate it too.  (The norm's node needs the statistics
+// and calls the inner operator: what a level further out would differentiate then is refused there.)
+std::vector<Tensor> norm_node(const Tensor& x, const Tensor& res, const Tensor& w, const Tensor& b, double eps, double rate,
+                              int64_t seed, const OptTensor& seed_at) {
     MAM_OP(op, layer_norm_forward);
-    const Tensor res = plain(residual), w = plain(weight), b = plain(bias);
-    if (!wants_grad(x, res, w, b)) return op.call(x, residual, weight, bias, eps, rate, seed, seed_at, false);
     auto node = make_node<NormBackward>(rate, seed, seed_at, x, res, w, b);
     std::vector<Tensor> out;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        out = op.call(x, residual, weight, bias, eps, rate, seed, seed_at, true);
+        out = op.call(x, opt(res), opt(w), opt(b), eps, rate, seed, seed_at, true);
     }
     node->stats = SavedVariable(out.back(), false);
     out.pop_back();
@@ -357,41 +382,108 @@ std::vector<Tensor> norm(const Tensor& x, const OptTensor& residual, const OptTe
     node->s = res.defined() ? SavedVariable(out[1], true) : SavedVariable(x, false);
     return out;
 }
+std::vector<Tensor> norm_plain(const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias,
+                               double eps, double rate, int64_t seed, const OptTensor& seed_at) {
+    MAM_OP(op, layer_norm_forward);
+    return op.call(x, residual, weight, bias, eps, rate, seed, seed_at, false);
+}
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
-    return norm(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt)[0];
+    const Tensor w = plain(weight), b = plain(bias);
+    refuse_tangents(x, w, b);
+    if (wants_grad(x, w, b)) return std::move(norm_node(x, Tensor(), w, b, eps, 0.0, 0, std::nullopt)[0]);
+    at::AutoDispatchBelowADInplaceOrView below;
+    if (transformed()) {
+        MAM_OP(self, layer_norm);
+        return self.call(x, weight, bias, eps);
+    }
+    return std::move(norm_plain(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt)[0]);
 }
 std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
                                                   const OptTensor& bias, double eps, double rate, int64_t seed,
                                                   const OptTensor& seed_at) {
-    auto out = norm(x, residual, weight, bias, eps, rate, seed, seed_at);
+    const Tensor w = plain(weight), b = plain(bias);
+    refuse_tangents(x, residual, w, b);
+    std::vector<Tensor> out;
+    if (wants_grad(x, residual, w, b)) {
+        out = norm_node(x, residual, w, b, eps, rate, seed, seed_at);
+    } else {
+        at::AutoDispatchBelowADInplaceOrView below;
+        if (transformed()) {
+            MAM_OP(self, dropout_add_layer_norm);
+            return self.call(x, residual, weight, bias, eps, rate, seed, seed_at);
+        }
+        out = norm_plain(x, residual, weight, bias, eps, rate, seed, seed_at);
+    }
     return {std::move(out[0]), std::move(out[1])};
 }
 Tensor dropout(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
     MAM_OP(op, dropout_forward);
+    MAM_OP(self, dropout);
     const Tensor res = plain(residual);
-    if (!wants_grad(x, res)) return op.call(x, residual, rate, seed, seed_at);
-    auto node = make_node<DropoutBackward>(rate, seed, seed_at, x, res);
+    refuse_tangents(x, res);
+    const auto node = wants_grad(x, res) ? make_node<DropoutBackward>(rate, seed, seed_at, x, res) : nullptr;
     Tensor y;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        y = op.call(x, residual, rate, seed, seed_at);
+        y = (transformed() ? self : op).call(x, residual, rate, seed, seed_at);
     }
-    torch::autograd::set_history(y, node);
+    if (node) torch::autograd::set_history(y, node);
     return y;
 }
 Tensor gelu(const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
     MAM_OP(op, gelu_forward);
-    if (!wants_grad(x)) return op.call(x, rate, seed, seed_at);
-    auto node = make_node<GeluBackward>(rate, seed, seed_at, x);
+    MAM_OP(self, gelu);
+    refuse_tangents(x);
+    const auto node = wants_grad(x) ? make_node<GeluBackward>(rate, seed, seed_at, x) : nullptr;
     Tensor y;
     {
         at::AutoDispatchBelowADInplaceOrView below;
-        y = op.call(x, rate, seed, seed_at);
+        y = (transformed() ? self : op).call(x, rate, seed, seed_at);
     }
-    node->x = SavedVariable(x, false);
-    torch::autograd::set_history(y, node);
+    if (node) {
+        node->x = SavedVariable(x, false);
+        torch::autograd::set_history(y, node);
+    }
     return y;
 }
+
+// The same operators below the autograd keys.
+Tensor layer_norm_below(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    return std::move(norm_plain(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt)[0]);
+}
+std::tuple<Tensor, Tensor> dropout_add_layer_norm_below(const Tensor& x, const Tensor& residual, const OptTensor& weight,
+                                                        const OptTensor& bias, double eps, double rate, int64_t seed,
+                                                        const OptTensor& seed_at) {
+    auto out = norm_plain(x, residual, weight, bias, eps, rate, seed, seed_at);
+    return {std::move(out[0]), std::move(out[1])};
+}
+Tensor dropout_below(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
+    MAM_OP(op, dropout_forward);
+    return op.call(x, residual, rate, seed, seed_at);
+}
+Tensor gelu_below(const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
+    MAM_OP(op, gelu_forward);
+    return op.call(x, rate, seed, seed_at);
+}
+
+// Eager calls from Python: straight to the functions above, under a transform by way of the dispatcher.
+template <class Fn, const char* NAME>
+struct Eager;
+template <class R, class... A, const char* NAME>
+struct Eager<R(A...), NAME> {
+    template <R (*FN)(A...)>
+    static R call(A... args) {
+        if (!transformed()) return FN(args...);
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<R(A...)>();
+        return op.call(args...);
+    }
+};
+
+constexpr char kNormForward[] = "mamtorch_b200::layer_norm_forward", kNormBackward[] = "mamtorch_b200::layer_norm_backward",
+               kDropoutForward[] = "mamtorch_b200::dropout_forward", kGeluForward[] = "mamtorch_b200::gelu_forward",
+               kGeluBackward[] = "mamtorch_b200::gelu_backward", kLayerNorm[] = "mamtorch_b200::layer_norm",
+               kAddNorm[] = "mamtorch_b200::dropout_add_layer_norm", kDropout[] = "mamtorch_b200::dropout",
+               kGelu[] = "mamtorch_b200::gelu";
 
 }  // namespace
 
@@ -401,10 +493,10 @@ TORCH_LIBRARY_FRAGMENT(mamtorch_b200, m) {
     m.def("dropout_forward(Tensor x, Tensor? residual, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
     m.def("gelu_forward(Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
     m.def("gelu_backward(Tensor gy, Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
-    m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor", &layer_norm);
-    m.def("dropout_add_layer_norm(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> (Tensor, Tensor)", &dropout_add_layer_norm);
-    m.def("dropout(Tensor x, Tensor? residual, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor", &dropout);
-    m.def("gelu(Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor", &gelu);
+    m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor");
+    m.def("dropout_add_layer_norm(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> (Tensor, Tensor)");
+    m.def("dropout(Tensor x, Tensor? residual, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("gelu(Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(mamtorch_b200, CUDA, m) {
     m.impl("layer_norm_forward", &layer_norm_forward);
@@ -414,12 +506,30 @@ TORCH_LIBRARY_IMPL(mamtorch_b200, CUDA, m) {
     m.impl("gelu_backward", &gelu_backward);
 }
 
+TORCH_LIBRARY_IMPL(mamtorch_b200, Autograd, m) {
+    m.impl("layer_norm_forward", &Inner<decltype(layer_norm_forward), kNormForward>::call);
+    m.impl("layer_norm_backward", &Inner<decltype(layer_norm_backward), kNormBackward>::call);
+    m.impl("dropout_forward", &Inner<decltype(dropout_forward), kDropoutForward>::call);
+    m.impl("gelu_forward", &Inner<decltype(gelu_forward), kGeluForward>::call);
+    m.impl("gelu_backward", &Inner<decltype(gelu_backward), kGeluBackward>::call);
+    m.impl("layer_norm", &layer_norm);
+    m.impl("dropout_add_layer_norm", &dropout_add_layer_norm);
+    m.impl("dropout", &dropout);
+    m.impl("gelu", &gelu);
+}
+TORCH_LIBRARY_IMPL(mamtorch_b200, CompositeExplicitAutograd, m) {
+    m.impl("layer_norm", &layer_norm_below);
+    m.impl("dropout_add_layer_norm", &dropout_add_layer_norm_below);
+    m.impl("dropout", &dropout_below);
+    m.impl("gelu", &gelu_below);
+}
+
 // The differentiable operators as plain functions of the module mamtorch_b200._C, for eager calls: the way through
 // torch.ops (a schema's arguments, boxed) takes a microsecond of the seven that a small call lasts.
 PYBIND11_MODULE(_C, m) {
     const pybind11::call_guard<pybind11::gil_scoped_release> free;
-    m.def("layer_norm", &layer_norm, free);
-    m.def("dropout_add_layer_norm", &dropout_add_layer_norm, free);
-    m.def("dropout", &dropout, free);
-    m.def("gelu", &gelu, free);
+    m.def("layer_norm", &Eager<decltype(layer_norm), kLayerNorm>::call<&layer_norm>, free);
+    m.def("dropout_add_layer_norm", &Eager<decltype(dropout_add_layer_norm), kAddNorm>::call<&dropout_add_layer_norm>, free);
+    m.def("dropout", &Eager<decltype(dropout), kDropout>::call<&dropout>, free);
+    m.def("gelu", &Eager<decltype(gelu), kGelu>::call<&gelu>, free);
 }
