@@ -194,6 +194,30 @@ def _(gy, x, drop_rate, drop_seed, drop_seed_at):
     return x.new_empty(x.shape)
 
 
+def _register_vmap(name):
+    """Under vmap the operators run sample by sample.  With one seed for all samples each would lose the same elements, since
+    a mask is a function of the seed and the element's number within its sample: refused."""
+    op = getattr(_ops, name).default
+    names = [a.name for a in op._schema.arguments]
+    rate, seed_at = (names.index(n) if n in names else None for n in ("drop_rate", "drop_seed_at"))
+
+    @torch.library.register_vmap(f"mamtorch_b200::{name}")
+    def _(info, in_dims, *args):
+        if rate is not None and args[rate] > 0 and in_dims[seed_at] is None:
+            raise RuntimeError(f"mamtorch_b200::{name} under vmap would drop the same elements in every sample: call it on the "
+                               "whole batch, or map over a tensor of seeds too")
+        outs = [op(*(a if d is None else a.select(d, i) for a, d in zip(args, in_dims))) for i in range(info.batch_size)]
+        if isinstance(outs[0], Tensor):
+            return torch.stack(outs), 0
+        kind = type(outs[0])
+        return kind(torch.stack(o) for o in zip(*outs)), kind(0 for _ in outs[0])
+
+
+for _op_name in ("layer_norm", "dropout_add_layer_norm", "dropout", "gelu", "layer_norm_forward", "layer_norm_backward",
+              "dropout_forward", "gelu_forward", "gelu_backward"):
+    _register_vmap(_op_name)
+
+
 @torch.library.register_fake("mamtorch_b200::dense_nt")
 def _(a, w):
     torch._check(a.dim() == 2 and w.dim() == 2 and a.size(1) == w.size(1))
@@ -468,7 +492,8 @@ def dropout_add_layer_norm(x: Tensor, residual: Tensor, weight: Tensor | None = 
 
 def dropout(x: Tensor, drop_rate: float, drop_seed=None, residual: Tensor | None = None) -> Tensor:
     """dropout(x), or residual + dropout(x), the mask formed from the seed forward and backward and never stored.  It
-    always drops (a training-time operator).  Its masks are not those of `weight_drop` and the MAM layers' output dropout:
+    always drops (a training-time operator), and is refused under vmap, where one seed would give all samples one mask, unless
+    the seeds are mapped over too.  Its masks are not those of `weight_drop` and the MAM layers' output dropout:
     it takes one 64-bit draw for two elements, they take one for each."""
     return (_C.dropout if _eager(x) else _ops.dropout.default)(x, residual, *_drop_args(drop_rate, drop_seed))
 

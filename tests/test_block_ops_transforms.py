@@ -176,3 +176,44 @@ def test_inner_operators_have_no_derivative_of_their_own(cpu_kernels):
                 *ops.layer_norm_forward(x, None, None, None, 1e-5, 0.0, 0, None, True)):
         with pytest.raises(RuntimeError, match="differentiable once"):
             out.sum().backward()
+
+
+# ---------------------------------------------------------------- vmap
+
+@pytest.mark.parametrize("name", [k for k in OPS if "drop" in k])
+def test_vmap_of_a_dropout_is_refused(cpu_kernels, name):
+    """One seed and the same element numbers: every sample would lose the same elements."""
+    f, _ = OPS[name]
+    xs = rand(4, 3, 6, seed=6)
+    for g in (f, torch.func.grad(lambda v: (f(v) * V).sum()), lambda v: torch.func.vmap(f)(v.unsqueeze(0)),
+              lambda v: torch.func.vjp(f, v)[1](V)[0]):
+        with pytest.raises(RuntimeError, match="same elements in every sample"):
+            torch.func.vmap(g)(xs)
+    with pytest.raises(RuntimeError, match="same elements in every sample"):
+        torch.func.vmap(lambda g: torch.ops.mamtorch_b200.dropout_forward(g, None, 0.5, 3, None))(xs)
+
+
+def test_vmap_without_a_dropout_goes_sample_by_sample(cpu_kernels):
+    xs, ws, bs = rand(4, 3, 6, seed=6), rand(4, 6, seed=7), rand(6, 4, seed=8)
+    cases = {
+        "gelu": (MF.gelu, (0,), (xs,)), "gelu, last": (MF.gelu, (1,), (xs.movedim(0, 1),)),
+        "dropout": (lambda v: MF.dropout(v, 0.0), (0,), (xs,)), "residual": (lambda v: MF.dropout(RES, 0.0, residual=v), (0,), (xs,)),
+        "layer_norm": (lambda v: MF.layer_norm(v, W, B), (0,), (xs,)), "weights": (lambda w, b: MF.layer_norm(RES, w, b), (0, 1), (ws, bs)),
+        "add": (lambda v, w: MF.dropout_add_layer_norm(v, RES, w, B), (0, 0), (xs, ws)),
+        "per-sample gradients": (torch.func.grad(lambda w, v: (MF.layer_norm(v, w, B) * V).sum()), (None, 0), (W, xs)),
+        "gelu's": (torch.func.grad(lambda v: (MF.gelu(v) * V).sum()), (0,), (xs,)),
+    }
+    for name, (f, dims, args) in cases.items():
+        got = torch.func.vmap(f, in_dims=dims)(*args)
+        want = [f(*(a if d is None else a.select(d, i) for a, d in zip(args, dims))) for i in range(4)]
+        for g, w in zip(got if isinstance(got, tuple) else (got,), zip(*want) if isinstance(want[0], tuple) else (want,)):
+            torch.testing.assert_close(g, torch.stack(w), **CLOSE, msg=name)
+
+
+def test_vmap_over_seeds_gives_each_sample_its_mask():
+    """Seeds in a tensor: the kernels get one a sample."""
+    seeds, x = torch.tensor([3, 4, 9]), rand(50, seed=1)
+    with torch.library._scoped_library("mamtorch_b200", "IMPL") as lib:
+        lib.impl("dropout_forward", lambda x, res, rate, seed, at: drop(x, rate, seed + int(at)), "CPU")
+        got = torch.func.vmap(lambda s: MF.dropout(x, 0.5, s))(seeds)
+    assert torch.equal(got, torch.stack([drop(x, 0.5, int(s)) for s in seeds]))
