@@ -545,12 +545,16 @@ int launch_bwd_split(const float* a, const float* b, const float* grad, const in
 }  // namespace
 
 int mamb200::wait_flag(int** flag) {
-    static int* known[64];        // a device's address never changes
+    static std::atomic<int*> known[64];        // a device's address never changes
     int dev = 0;
     MAM_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
-    if (!known[dev]) MAM_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&known[dev]), g_wait_gave_up));
-    *flag = known[dev];
+    int* at = known[dev].load(std::memory_order_relaxed);
+    if (!at) {
+        MAM_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&at), g_wait_gave_up));
+        known[dev].store(at, std::memory_order_relaxed);
+    }
+    *flag = at;
     return MAM_OK;
 }
 

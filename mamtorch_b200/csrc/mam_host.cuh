@@ -1,6 +1,8 @@
 // Host-side helpers shared by the translation units of libmam_b200.so: error recording and device attributes.
 #pragma once
+#include <atomic>
 #include <cuda_runtime.h>
+#include <mutex>
 
 #include "../../include/mam_b200.h"
 
@@ -19,21 +21,28 @@ inline int cuda_fail(cudaError_t e) {
     } while (0)
 
 struct DevInfo {
-    int valid = 0, sms = 0, major = 0, minor = 0, max_smem = 0;
+    int sms = 0, major = 0, minor = 0, max_smem = 0;
 };
 inline DevInfo g_dev[64];
+inline std::atomic<bool> g_dev_known[64];     // written behind the mutex: calls come from any thread
+inline std::mutex g_dev_mutex;
 
 inline int device_info(const DevInfo** out) {
     int dev = 0;
     MAM_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
     DevInfo& d = g_dev[dev];
-    if (!d.valid) {
-        MAM_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
-        MAM_CUDA(cudaDeviceGetAttribute(&d.major, cudaDevAttrComputeCapabilityMajor, dev));
-        MAM_CUDA(cudaDeviceGetAttribute(&d.minor, cudaDevAttrComputeCapabilityMinor, dev));
-        MAM_CUDA(cudaDeviceGetAttribute(&d.max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev));
-        d.valid = 1;
+    if (!g_dev_known[dev].load(std::memory_order_acquire)) {
+        std::lock_guard<std::mutex> lock(g_dev_mutex);
+        DevInfo n;
+        MAM_CUDA(cudaDeviceGetAttribute(&n.sms, cudaDevAttrMultiProcessorCount, dev));
+        MAM_CUDA(cudaDeviceGetAttribute(&n.major, cudaDevAttrComputeCapabilityMajor, dev));
+        MAM_CUDA(cudaDeviceGetAttribute(&n.minor, cudaDevAttrComputeCapabilityMinor, dev));
+        MAM_CUDA(cudaDeviceGetAttribute(&n.max_smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev));
+        if (!g_dev_known[dev].load(std::memory_order_relaxed)) {
+            d = n;
+            g_dev_known[dev].store(true, std::memory_order_release);
+        }
     }
     *out = &d;
     return d.major == 10 ? MAM_OK : MAM_ERR_NOT_SM100;

@@ -1,0 +1,65 @@
+"""Layer norm, dropout and GELU operators: first calls of a process, copies of modules, waits that run out, what GELU's form is worth
+in fp32."""
+import copy
+import os
+import subprocess
+import sys
+import textwrap
+
+import pytest
+import torch
+
+from conftest import ROOT
+
+pytestmark = pytest.mark.gpu
+
+
+def fresh_process(code, *args):
+    """Runs a program in a process of its own, from the repository's root; its output."""
+    env = dict(os.environ, PYTHONPATH=ROOT)
+    run = subprocess.run([sys.executable, "-c", textwrap.dedent(code), *args], cwd=ROOT, env=env, capture_output=True, text=True,
+                         timeout=300)
+    assert run.returncode == 0, run.stdout + run.stderr
+    return run.stdout
+
+
+def test_first_calls_from_several_threads(cuda):
+    """Nothing of the library has run in the process yet: each thread may be the one that asks for a device's attributes, a
+    kernel's shared memory or the flag's address.  Every width in every type, rows enough for the forward's ring."""
+    out = fresh_process("""
+        import threading
+        from concurrent.futures import ThreadPoolExecutor
+        import torch
+        from mamtorch_b200.nn import functional as MF
+
+        CASES = [(rows, width, t) for rows, width in ((300, 200), (2400, 1283), (300, 2500), (2400, 4096), (300, 7000), (64, 9000),
+                                                      (2400, 1000), (300, 8192))
+                 for t in (torch.float32, torch.bfloat16, torch.float16)]
+        torch.cuda.init()
+        start = threading.Barrier(8)
+
+        def work(k, wait):
+            rows, width, t = CASES[k]
+            g = torch.Generator().manual_seed(k)
+            x, r, gy = (torch.randn(rows, width, generator=g).to(t).cuda() for _ in range(3))
+            x.requires_grad_()
+            w, b = (torch.randn(width, generator=g).to(t).cuda().requires_grad_() for _ in range(2))
+            torch.cuda.synchronize()
+            if wait:
+                start.wait(60)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                y, s = MF.dropout_add_layer_norm(MF.gelu(x, 0.1, k), r, w, b, 1e-5, 0.1, k)
+                z = MF.layer_norm(x, w, b)
+                out = [y, s, z, *torch.autograd.grad((y, s, z), (x, w, b), (gy, gy, gy))]
+                torch.cuda.current_stream().synchronize()
+            return out
+
+        with ThreadPoolExecutor(8) as pool:
+            at_once = list(pool.map(lambda k: work(k, True), range(len(CASES))))
+        for k, got in enumerate(at_once):
+            for p, q in zip(got, work(k, False)):
+                assert torch.equal(p, q), CASES[k]
+        MF.check_device_flag()
+        print("same")
+    """)
+    assert out.strip() == "same"
