@@ -15,9 +15,12 @@ pytestmark = pytest.mark.gpu
 
 
 def fresh_process(code, *args):
-    """Runs a program in a process of its own, from the repository's root; its output."""
+    """Runs a program in a process of its own, from the repository's root; its output.  The process leaves without the
+    interpreter's teardown, where torch's engine threads may abort it after backward passes from several threads (with
+    torch's own operators too)."""
     env = dict(os.environ, PYTHONPATH=ROOT)
-    run = subprocess.run([sys.executable, "-c", textwrap.dedent(code), *args], cwd=ROOT, env=env, capture_output=True, text=True,
+    code = textwrap.dedent(code) + "\nimport os, sys\nsys.stdout.flush()\nos._exit(0)\n"
+    run = subprocess.run([sys.executable, "-c", code, *args], cwd=ROOT, env=env, capture_output=True, text=True,
                          timeout=300)
     assert run.returncode == 0, run.stdout + run.stderr
     return run.stdout
