@@ -91,8 +91,8 @@ def vcon_step_all(model: nn.Module) -> None:
 
 class _DropSeeds(nn.Module):
     """Seeds for the dropout of a module.  Eagerly they are numbers from torch's CPU generator.  Inside a graph capture a
-    number would repeat one mask at every replay, so there a device counter is advanced and copied, which the graph does
-    again each time it runs."""
+    number would repeat one mask at every replay, so there a device counter is advanced, which the graph does again each
+    time it runs, and a number drawn at the capture is added: deep copies of a module copy its counter."""
 
     def __init__(self, device=None):
         super().__init__()
@@ -103,7 +103,7 @@ class _DropSeeds(nn.Module):
         if not (self.counter.is_cuda and torch.cuda.is_current_stream_capturing()):
             return MF.fresh_drop_seed()
         self.counter.add_(0x632BE59BD9B4E019)
-        return self.counter.clone()
+        return self.counter + MF.fresh_drop_seed()
 
 
 class MAMMlpBlock(nn.Module):

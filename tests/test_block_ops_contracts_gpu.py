@@ -66,3 +66,29 @@ def test_first_calls_from_several_threads(cuda):
         print("same")
     """)
     assert out.strip() == "same"
+
+
+def test_copies_of_a_module_drop_their_own_elements_in_a_captured_graph(cuda):
+    """In a capture the seeds come from a device counter, which a deep copy of the module copies."""
+    from mamtorch_b200.nn.vit import MAMMlpBlock
+
+    torch.manual_seed(0)
+    block = MAMMlpBlock(64, 128, fused=True, drop_rate=0.5).to(cuda)
+    twins = [block, copy.deepcopy(block), copy.deepcopy(block)]
+    x = torch.randn(40, 64, device=cuda)
+    with torch.no_grad():
+        for twin in twins:
+            twin(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [twin(x) for twin in twins]
+            seeds = [twin.drop_args()[1] for twin in twins]
+    seen = []
+    for _ in range(3):
+        graph.replay()
+        # where the last dropout dropped, the output is the input
+        masks = [y == x for y in outs]
+        assert not any(torch.equal(masks[i], masks[j]) for i in range(3) for j in range(i))
+        seen += [int(s) for s in seeds]
+    assert len(set(seen)) == 9
