@@ -48,6 +48,8 @@ inline int device_info(const DevInfo** out) {
     return d.major == 10 ? MAM_OK : MAM_ERR_NOT_SM100;
 }
 
+inline int g_norm_wait = -1;  // polls of the norm's ring (MAM_TUNE_NORM_WAIT), or -1: the constant
+
 int wait_flag(int** flag);    // device address of the flag that kernels set when a bounded wait runs out (mam_capi.cu)
 
 inline int bad_ptr(const void* p) { return p == nullptr; }

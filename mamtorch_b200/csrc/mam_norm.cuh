@@ -218,7 +218,42 @@ struct NormRing {
     int group, groups, stages;
     unsigned slot_bytes;                   // of one tensor's row
     unsigned weights_at, bars_at, bytes;   // the parameters, the barriers; the whole
+    unsigned polls;                        // of a wait for a row, after which it gives up
 };
+
+// The barrier of a row's group, with a vote: whether any of its threads says so.  All of them get the same answer.
+__device__ __forceinline__ bool group_any(int g, int group, bool mine) {
+    if (group == 32) {
+        __syncwarp();
+        return __any_sync(~0u, mine);
+    }
+    unsigned any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %3, 0;\n\t"
+        "bar.red.or.pred q, %1, %2, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(any)
+        : "r"(g + 1), "r"(group), "r"((unsigned)mine)
+        : "memory");
+    return any != 0;
+}
+
+// What a group does when a wait for a row ran out, as the vote behind it tells all its threads: the results are void, the flag
+// says so, and the group leaves its loop without arming a barrier or sending for a row again.  The copies that are on
+// their way, of `sent` rows from `row` on, write to this CTA's shared memory and are waited for (at length, one thread)
+// before the CTA may reuse or leave it.
+__device__ __forceinline__ void ring_give_up(uint64_t* full, int stages, int stage, unsigned phase, int sent, long long row,
+                                             long long step, long long rows, int* flag) {
+    *flag = 1;
+    for (int k = 0; k < sent && row < rows; ++k, row += step) {
+        mbar_wait_bounded(full + stage, phase);
+        if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+}
 
 // Many rows that are ragged, or too wide for the next kernel's loads to be held: one CTA an SM walks them with the parameters
 // in shared memory, in fp32.  A group's row leaves its stage for the
@@ -292,13 +327,9 @@ mam_norm_fwd_ring_kernel(const __grid_constant__ NormFwdParams p, const __grid_c
     uint4 carry = make_uint4(0u, 0u, 0u, 0u);
     int stage = 0;
     unsigned phase = 0;
-    bool lost = false;
     for (; row < p.rows; row += step, at += at_step, start += drop_step) {
         unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
-        if (!mbar_wait_bounded(full + stage, phase, lost ? 1024 : 1u << 22)) {
-            lost = true;            // the results are void, but every barrier is still met and every copy waited for
-            *p.wait_flag = 1;
-        }
+        const bool late = !mbar_wait_bounded(full + stage, phase, ring.polls);
         unsigned skip_x = 0, skip_r = 0;
         if constexpr (MODE == RAGGED) {
             const T *px = x0 + row * p.x_pitch, *pr = r0 + row * p.res_pitch;
@@ -341,7 +372,10 @@ mam_norm_fwd_ring_kernel(const __grid_constant__ NormFwdParams p, const __grid_c
         }
         float mu = lane_sum<32>(sum2(s));
         if (warps > 1 && lane == 0) slot[0][threadIdx.x >> 5].x = mu;
-        meet();
+        if (group_any(g, group, late)) {
+            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages, row, step, p.rows, p.wait_flag);
+            break;
+        }
         // all have this row in their registers
         if (t == 0) send(row + ring.stages * step, stage);
         if (warps > 1) mu = lane_sum<MOST>(lane < warps ? slot[0][slot0 + lane].x : 0.f);
@@ -694,10 +728,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
         if (row + step < p.rows) next = p.stats[row + step];
         const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
         const unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
-        if (!mbar_wait_bounded(full + stage, phase, lost ? 1024 : 1u << 22)) {
-            lost = true;            // the results are void, but every barrier is still met and every copy waited for
-            *p.wait_flag = 1;
-        }
+        const bool late = !mbar_wait_bounded(full + stage, phase, ring.polls);
         float2 h[NV][V / 2], a[NV][V / 2], s1 = splat2(0.f), s2 = s1;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -728,12 +759,12 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
                 }
             }
         float2 m = lane_sum2<32>(sum2(s1), sum2(s2));
-        if (warps > 1) {
-            // two sets of slots in turn: a set is written again only behind the next row's barrier
-            if (lane == 0) slot[parity][threadIdx.x >> 5] = m;
-            asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
-        } else {
-            __syncwarp();
+        // two sets of slots in turn: a set is written again only behind the next row's barrier
+        if (warps > 1 && lane == 0) slot[parity][threadIdx.x >> 5] = m;
+        if (group_any(g, group, late)) {
+            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait_flag);
+            lost = true;
+            break;
         }
         // all have left the row before this one: its stage takes the row stages - 1 ahead
         if (t == 0) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
@@ -774,8 +805,8 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
     }
     if (!p.partial) return;
     float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
-    // the groups' sums meet in the ring's memory, where no copy is on its way any more: a fixed order
-    __syncthreads();
+    // the groups' sums meet in the ring's memory, where no copy is on its way any more (unless a wait gave up): a fixed order
+    if (__syncthreads_or(lost)) return;
     float* cols = reinterpret_cast<float*>(smem);
     float* to = groups > 1 ? cols + (size_t)g * 2 * width : out;
 #pragma unroll
@@ -885,10 +916,7 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
         if (row + step < p.rows) next = p.stats[row + step];
         const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
         unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
-        if (!mbar_wait_bounded(full + stage, phase, lost ? 1024 : 1u << 22)) {
-            lost = true;            // the results are void, but every barrier is still met and every copy waited for
-            *p.wait_flag = 1;
-        }
+        const bool late = !mbar_wait_bounded(full + stage, phase, ring.polls);
         const T *ps = s0 + row * p.s_pitch, *py = gy0 + at, *pz = gs0 + at;
         if (edge(row)) {
             T *ds = reinterpret_cast<T*>(from + misfit(ps)), *dy = reinterpret_cast<T*>(from + ring.slot_bytes + misfit(py)),
@@ -940,7 +968,11 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
         float2 m = lane_sum2<32>(sum2(s1), sum2(s2));
         // two sets of slots in turn: a set is written again only behind the next row's barrier
         if (warps > 1 && lane == 0) slot[parity][threadIdx.x >> 5] = m;
-        meet();
+        if (group_any(g, group, late)) {
+            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait_flag);
+            lost = true;
+            break;
+        }
         // all have left the row before this one: its stage takes the row stages - 1 ahead
         if (t == 0) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
         if (warps > 1) {
@@ -990,8 +1022,8 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
     }
     if (!p.partial) return;
     float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
-    // the groups' sums meet in the ring's memory, where no copy is on its way any more: a fixed order
-    __syncthreads();
+    // the groups' sums meet in the ring's memory, where no copy is on its way any more (unless a wait gave up): a fixed order
+    if (__syncthreads_or(lost)) return;
     float* cols = reinterpret_cast<float*>(smem);
     float* to = groups > 1 ? cols + (size_t)g * 2 * width : out;
 #pragma unroll

@@ -92,3 +92,77 @@ def test_copies_of_a_module_drop_their_own_elements_in_a_captured_graph(cuda):
         assert not any(torch.equal(masks[i], masks[j]) for i in range(3) for j in range(i))
         seen += [int(s) for s in seeds]
     assert len(set(seen)) == 9
+
+
+@pytest.fixture
+def ring_wait():
+    """Sets after how many polls a norm's wait for a row gives up; the library's own limit afterwards."""
+    from mamtorch_b200 import _lib
+
+    L = _lib.lib()
+    yield lambda polls: _lib.check(L.mam_tune_set(6, polls), "mam_tune_set")
+    _lib.check(L.mam_tune_set(6, -1), "mam_tune_set")
+    L.mam_check_device_flag()
+
+
+# rows through shared memory: by columns one or several rows at a time in a CTA, aligned and ragged; many rows a group, and few
+RING_SHAPES = [(3000, 131), (3000, 1283), (2400, 8191), (3000, 136), (3000, 768), (20, 1024), (2400, 4096), (2500, 8192), (1, 200)]
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", RING_SHAPES)
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable(cuda, ring_wait, shape, t):
+    """Limits of no poll (every group gives up at its first row, with its copies on their way) and of one (at any row, or at
+    none)."""
+    from mamtorch_b200.nn import functional as MF
+
+    rows, width = shape
+    x, r, gy = (torch.randn(rows, width, device=cuda).to(t) for _ in range(3))
+    x.requires_grad_()
+    w, b = (torch.randn(width, device=cuda).to(t).requires_grad_() for _ in range(2))
+
+    def step():
+        y, s = MF.dropout_add_layer_norm(x, r, w, b, 1e-5, 0.1, 5)
+        z = MF.layer_norm(x, w, b)
+        return [y, s, z, *torch.autograd.grad((y, s, z), (x, w, b), (gy, gy, gy))]
+
+    want = step()
+    MF.check_device_flag()
+    for polls in (0, 1, 0, 1):
+        y, s = MF.dropout_add_layer_norm(x, r, w, b, 1e-5, 0.1, 5)      # the forward's wait is the library's own
+        z = MF.layer_norm(x, w, b)
+        ring_wait(polls)
+        grads = torch.autograd.grad((y, s, z), (x, w, b), (gy, gy, gy))
+        try:
+            MF.check_device_flag()
+            assert polls > 0
+            assert all(torch.equal(p, q) for p, q in zip(grads, want[3:]))
+        except RuntimeError as e:
+            assert "gave up" in str(e)
+        out = step()
+        try:
+            MF.check_device_flag()
+            assert polls > 0
+            assert all(torch.equal(p, q) for p, q in zip(out, want))
+        except RuntimeError as e:
+            assert "gave up" in str(e)
+        ring_wait(-1)
+        assert all(torch.equal(p, q) for p, q in zip(step(), want))
+        MF.check_device_flag()
+
+
+def test_a_forward_whose_wait_runs_out_is_reported(cuda, ring_wait):
+    from mamtorch_b200.nn import functional as MF
+
+    # ragged rows, and wide 16-bit ones behind a residual: the forward's forms through shared memory
+    for shape, t, add in (((3000, 1283), torch.bfloat16, False), ((3000, 201), torch.float32, True), ((2400, 4096), torch.float16, True)):
+        x, r = (torch.randn(shape, device=cuda).to(t) for _ in range(2))
+        call = (lambda: MF.dropout_add_layer_norm(x, r, drop_rate=0.1, drop_seed=5)) if add else (lambda: (MF.layer_norm(x),))   # noqa: B023
+        want = call()
+        ring_wait(0)
+        call()
+        with pytest.raises(RuntimeError, match="gave up"):
+            MF.check_device_flag()
+        ring_wait(-1)
+        assert all(torch.equal(p, q) for p, q in zip(call(), want))
+        MF.check_device_flag()
