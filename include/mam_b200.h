@@ -50,9 +50,10 @@ int mam_check_device_flag(void);
 
 /* The same check without waiting for the device, for callers that must not stall their stream: returns
  * MAM_ERR_DEVICE_TIMEOUT if the copy of the flag that an EARLIER call of this function fetched shows a
- * wait that ran out (and then clears flag and copy), else queues the next fetch of the flag on `stream`
- * (4 bytes into pinned host memory the library keeps per device) and returns MAM_OK.  A time-out is thus
- * reported one call late at most.  No counterpart in the reference, whose kernels have no bounded waits. */
+ * wait that ran out (and then clears flag and copy; the layer norm's kernels set the copy by themselves),
+ * else queues the next fetch of the flag on `stream` (4 bytes into pinned host memory the library keeps per
+ * device) and returns MAM_OK.  A time-out is thus reported one call late at most.  No counterpart in the
+ * reference, whose kernels have no bounded waits. */
 int mam_poll_device_flag(void* stream);
 
 /* Per-kernel timing without a profiler.  While armed, every launch of the kernel class `kernel_id`
@@ -395,7 +396,8 @@ int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int
  * NULL (zeros).  ds: gradient of s, which is the residual's too.  dx, required where drop_rate > 0: drop(ds), the gradient
  * of x; else optional, and equal to ds.  dweight and dbias, each optional, in param_dtype: summed in a fixed order;
  * with either of them the call needs the workspace (256-byte aligned).  Rows travel through shared memory under bounded
- * waits (mam_check_device_flag), in the forward for some shapes too. */
+ * waits, in the forward for some shapes too: one that ran out is reported by the next call of either function on the device
+ * that finds it (MAM_ERR_DEVICE_TIMEOUT, nothing is launched then; not inside a capture), or by mam_check_device_flag. */
 size_t mam_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t width);
 int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t s_pitch, const float* stats,
                        const void* weight, int param_dtype,

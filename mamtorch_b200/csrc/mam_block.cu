@@ -149,7 +149,7 @@ int fwd_pick(NormFwdParams& p, bool aligned, const DevInfo& d, cudaStream_t st) 
     if ((!aligned || (ADD && eight && sizeof(T) == 2)) && p.rows >= 16LL * d.sms && p.width > 128) {
         const FwdPlan b = fwd_plan(p.width, sizeof(T), ADD, aligned, d);
         if (b.per) {
-            const int e = wait_flag(&p.wait_flag);
+            const int e = wait_words(&p.wait);
             if (e != MAM_OK) return e;
             if (b.per == 8) return fwd_ring<T, 8 / VEC<T>, ADD>(p, b, aligned, d, st);
             if (b.per == 16) return fwd_ring<T, 16 / VEC<T>, ADD>(p, b, aligned, d, st);
@@ -381,11 +381,12 @@ int mam_layer_norm_fwd(const void* x, int64_t x_pitch, const void* residual, int
         return MAM_ERR_INVALID_ARGUMENT;
     if (rows > MOST_ROWS || width > MOST_WIDTH) return MAM_ERR_UNSUPPORTED;
     NormFwdParams p{x, residual, weight, bias, y, sum, reinterpret_cast<float2*>(stats), rows, width, x_pitch,
-                    residual_pitch, eps, 1.0f / (float)width, param_dtype == MAM_F32, nullptr, {}};
+                    residual_pitch, eps, 1.0f / (float)width, param_dtype == MAM_F32, {}, {}};
     int st = drop_args(drop_rate, drop_seed, drop_seed_at, &p.drop);
     if (st != MAM_OK) return st;
     const DevInfo* d = nullptr;
     st = device_info(&d);
+    if (st == MAM_OK) st = report_wait((cudaStream_t)stream);      // of an earlier call
     if (st != MAM_OK) return st;
     const int per = 16 / dtype_size(dtype);
     const bool vec = width % per == 0 && x_pitch % per == 0 && (!residual || residual_pitch % per == 0) && aligned16(x) &&
@@ -422,11 +423,12 @@ int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t 
     if (rows > MOST_ROWS || width > MOST_WIDTH) return MAM_ERR_UNSUPPORTED;
     const bool want_params = dweight || dbias;
     NormBwdParams p{gy, gsum, s, reinterpret_cast<const float2*>(stats), weight, ds, dx, nullptr, rows, width, s_pitch,
-                    1.0f / (float)width, param_dtype == MAM_F32, nullptr, {}};
+                    1.0f / (float)width, param_dtype == MAM_F32, {}, {}};
     int st = drop_args(drop_rate, drop_seed, drop_seed_at, &p.drop);
     if (st != MAM_OK) return st;
     const DevInfo* d = nullptr;
     st = device_info(&d);
+    if (st == MAM_OK) st = report_wait((cudaStream_t)stream);      // of an earlier call
     if (st != MAM_OK) return st;
     const int per = 16 / dtype_size(dtype);
     const bool vec = width % per == 0 && s_pitch % per == 0 && aligned16(gy) && aligned16(gsum) && aligned16(s) &&
@@ -434,7 +436,7 @@ int mam_layer_norm_bwd(const void* gy, const void* gsum, const void* s, int64_t 
     const bool add = gsum || dx;
     const BwdPlan b = bwd_plan(rows, width, dtype_size(dtype), add, vec, *d);
     if (b.kind == BwdPlan::RING) {
-        st = wait_flag(&p.wait_flag);
+        st = wait_words(&p.wait);
         if (st != MAM_OK) return st;
     }
     if (want_params) {

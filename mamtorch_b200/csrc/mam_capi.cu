@@ -544,18 +544,63 @@ int launch_bwd_split(const float* a, const float* b, const float* grad, const in
 }
 }  // namespace
 
-int mamb200::wait_flag(int** flag) {
-    static std::atomic<int*> known[64];        // a device's address never changes
-    int dev = 0;
-    MAM_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
-    int* at = known[dev].load(std::memory_order_relaxed);
-    if (!at) {
-        MAM_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&at), g_wait_gave_up));
-        known[dev].store(at, std::memory_order_relaxed);
-    }
-    *flag = at;
+namespace {
+// A device's words, which never move: looked up at their first use by any thread, in a capture too.
+std::atomic<int*> g_wait_flag[64], g_wait_image[64];
+std::mutex g_wait_mutex;
+
+int device_index(int* dev) {
+    MAM_CUDA(cudaGetDevice(dev));
+    return *dev >= 0 && *dev < 64 ? MAM_OK : MAM_ERR_UNSUPPORTED;
+}
+int look_up(int dev) {
+    int *flag = nullptr, *image = nullptr;
+    MAM_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&flag), g_wait_gave_up));
+    MAM_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&image), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+    *image = 0;
+    g_wait_flag[dev].store(flag, std::memory_order_relaxed);
+    g_wait_image[dev].store(image, std::memory_order_release);
     return MAM_OK;
+}
+int clear_wait(int dev) {
+    const int zero = 0;
+    MAM_CUDA(cudaMemcpyToSymbol(g_wait_gave_up, &zero, sizeof(int)));
+    if (int* image = g_wait_image[dev].load(std::memory_order_acquire)) *reinterpret_cast<volatile int*>(image) = 0;
+    return MAM_OK;
+}
+}  // namespace
+
+int mamb200::wait_words(WaitWords* w) {
+    int dev = 0;
+    int st = device_index(&dev);
+    if (st != MAM_OK) return st;
+    if (!g_wait_image[dev].load(std::memory_order_acquire)) {
+        std::lock_guard<std::mutex> lock(g_wait_mutex);
+        if (!g_wait_image[dev].load(std::memory_order_acquire)) {
+            // pinned memory is not to be had inside a capture unless the thread says that it knows
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            MAM_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+            st = look_up(dev);
+            MAM_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+            if (st != MAM_OK) return st;
+        }
+    }
+    w->flag = g_wait_flag[dev].load(std::memory_order_relaxed);
+    w->image = g_wait_image[dev].load(std::memory_order_relaxed);
+    return MAM_OK;
+}
+
+int mamb200::report_wait(cudaStream_t stream) {
+    int dev = 0;
+    int st = device_index(&dev);
+    if (st != MAM_OK) return st;
+    const int* image = g_wait_image[dev].load(std::memory_order_acquire);
+    if (!image || !*reinterpret_cast<const volatile int*>(image)) return MAM_OK;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    MAM_CUDA(cudaStreamIsCapturing(stream, &cap));
+    if (cap != cudaStreamCaptureStatusNone) return MAM_OK;
+    st = clear_wait(dev);      // may wait for the device
+    return st != MAM_OK ? st : MAM_ERR_DEVICE_TIMEOUT;
 }
 
 extern "C" {
@@ -584,38 +629,22 @@ int mam_check_device_flag(void) {
     MAM_CUDA(cudaDeviceSynchronize());
     int flag = 0;
     MAM_CUDA(cudaMemcpyFromSymbol(&flag, g_wait_gave_up, sizeof(int)));
-    if (flag) {
-        int zero = 0;
-        MAM_CUDA(cudaMemcpyToSymbol(g_wait_gave_up, &zero, sizeof(int)));
-        return MAM_ERR_DEVICE_TIMEOUT;
-    }
-    return MAM_OK;
+    if (!flag) return MAM_OK;
+    int dev = 0, st = device_index(&dev);
+    if (st == MAM_OK) st = clear_wait(dev);
+    return st != MAM_OK ? st : MAM_ERR_DEVICE_TIMEOUT;
 }
 
 int mam_poll_device_flag(void* stream) {
-    int dev = 0;
-    MAM_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64) return MAM_ERR_UNSUPPORTED;
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     MAM_CUDA(cudaStreamIsCapturing((cudaStream_t)stream, &cap));
     if (cap != cudaStreamCaptureStatusNone) return MAM_OK;   // nothing is fetched or reported inside a capture
-    // one pinned int per device: the landing place of the asynchronous fetches
-    static int* mirror[64] = {nullptr};
-    if (mirror[dev] == nullptr) {
-        int* p = nullptr;
-        MAM_CUDA(cudaHostAlloc(reinterpret_cast<void**>(&p), sizeof(int), cudaHostAllocDefault));
-        *p = 0;
-        mirror[dev] = p;
-    }
-    const int seen = *reinterpret_cast<volatile int*>(mirror[dev]);
-    if (seen) {
-        // report once: clear the device flag and the copy (this path may wait for the device)
-        int zero = 0;
-        MAM_CUDA(cudaMemcpyToSymbol(g_wait_gave_up, &zero, sizeof(int)));
-        *mirror[dev] = 0;
-        return MAM_ERR_DEVICE_TIMEOUT;
-    }
-    MAM_CUDA(cudaMemcpyFromSymbolAsync(mirror[dev], g_wait_gave_up, sizeof(int), 0, cudaMemcpyDeviceToHost,
+    WaitWords w;
+    int st = wait_words(&w);
+    if (st != MAM_OK) return st;
+    st = report_wait((cudaStream_t)stream);
+    if (st != MAM_OK) return st;
+    MAM_CUDA(cudaMemcpyFromSymbolAsync(w.image, g_wait_gave_up, sizeof(int), 0, cudaMemcpyDeviceToHost,
                                        (cudaStream_t)stream));
     return MAM_OK;
 }

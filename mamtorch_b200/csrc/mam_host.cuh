@@ -50,7 +50,14 @@ inline int device_info(const DevInfo** out) {
 
 inline int g_norm_wait = -1;  // polls of the norm's ring (MAM_TUNE_NORM_WAIT), or -1: the constant
 
-int wait_flag(int** flag);    // device address of the flag that kernels set when a bounded wait runs out (mam_capi.cu)
+// Where kernels say that a bounded wait ran out (mam_capi.cu): a flag of the device, and its image in pinned host memory, which
+// kernels that are given its address write too, so that the host sees it without a copy.
+struct WaitWords {
+    int *flag, *image;
+};
+int wait_words(WaitWords* w);
+// MAM_ERR_DEVICE_TIMEOUT, once, where the image of the current device says so and `stream` is not being captured
+int report_wait(cudaStream_t stream);
 
 inline int bad_ptr(const void* p) { return p == nullptr; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -13,6 +13,7 @@
 // mean first and the deviations from it second, so that a mean far from zero costs no digits.
 #pragma once
 #include "mam_drop.cuh"
+#include "mam_host.cuh"
 #include "mam_ptx.cuh"
 #include "mam_vec.cuh"
 
@@ -33,7 +34,7 @@ struct NormFwdParams {
     long long rows, width, x_pitch, res_pitch;
     float eps, inv_width;
     bool params_f32;
-    int* wait_flag;            // set where a bounded wait ran out
+    WaitWords wait;            // set where a bounded wait ran out
     DropArgs drop;
 };
 
@@ -49,7 +50,7 @@ struct NormBwdParams {
     long long rows, width, s_pitch;
     float inv_width;
     bool params_f32;
-    int* wait_flag;            // set where a bounded wait ran out
+    WaitWords wait;            // set where a bounded wait ran out
     DropArgs drop;
 };
 
@@ -244,8 +245,10 @@ __device__ __forceinline__ bool group_any(int g, int group, bool mine) {
 // their way, of `sent` rows from `row` on, write to this CTA's shared memory and are waited for (at length, one thread)
 // before the CTA may reuse or leave it.
 __device__ __forceinline__ void ring_give_up(uint64_t* full, int stages, int stage, unsigned phase, int sent, long long row,
-                                             long long step, long long rows, int* flag) {
-    *flag = 1;
+                                             long long step, long long rows, const WaitWords& w) {
+    *w.flag = 1;
+    *reinterpret_cast<volatile int*>(w.image) = 1;
+    __threadfence_system();
     for (int k = 0; k < sent && row < rows; ++k, row += step) {
         mbar_wait_bounded(full + stage, phase);
         if (++stage == stages) {
@@ -373,7 +376,7 @@ mam_norm_fwd_ring_kernel(const __grid_constant__ NormFwdParams p, const __grid_c
         float mu = lane_sum<32>(sum2(s));
         if (warps > 1 && lane == 0) slot[0][threadIdx.x >> 5].x = mu;
         if (group_any(g, group, late)) {
-            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages, row, step, p.rows, p.wait_flag);
+            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages, row, step, p.rows, p.wait);
             break;
         }
         // all have this row in their registers
@@ -762,7 +765,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
         // two sets of slots in turn: a set is written again only behind the next row's barrier
         if (warps > 1 && lane == 0) slot[parity][threadIdx.x >> 5] = m;
         if (group_any(g, group, late)) {
-            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait_flag);
+            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait);
             lost = true;
             break;
         }
@@ -969,7 +972,7 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
         // two sets of slots in turn: a set is written again only behind the next row's barrier
         if (warps > 1 && lane == 0) slot[parity][threadIdx.x >> 5] = m;
         if (group_any(g, group, late)) {
-            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait_flag);
+            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait);
             lost = true;
             break;
         }

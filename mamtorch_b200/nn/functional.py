@@ -452,6 +452,8 @@ def selection_count_update_(count: Tensor, argmax: Tensor, argmin: Tensor, hits=
 # one int64 on the activations' device, which the kernels read when they run: a captured graph replays with a new mask
 # after the tensor was advanced.  The backward reads it again, so it must not change between a forward and its backward
 # (autograd raises if it did).
+# Rows may reach the norm's kernels under a bounded wait: should one run out, the next call of a norm, forward or backward,
+# outside a capture raises and launches nothing; after the last one `check_device_flag` does.
 
 def _eager(x) -> bool:
     """Whether the call may go to the C++ function itself: tracing and tensors with their own dispatch take the registered
