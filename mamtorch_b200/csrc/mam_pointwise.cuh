@@ -22,10 +22,18 @@ struct PointParams {
 enum PointOp { POINT_DROPOUT, POINT_GELU, POINT_GELU_BWD };
 
 // q = -erfc(a / sqrt(2)) / 2 and e = exp(-a^2 / 2) for a = min(|x|, 15), pairwise: the form of Abramowitz and Stegun, 7.1.26,
-// t P(t) e with t = 1 / (1 + 0.28 a), P with six coefficients of our own fit instead of five (largest error of the fit
-// 9.3e-9; in fp32 1.9e-7 at a = 0, where the roundings of the sum to 0.5 count, and 6.3e-8 for a q).  erff and expf took
-// 33 instructions an element and twice the time of the bytes in bf16; this takes a reciprocal, an exponential and the
-// rest in packed pairs.  15: beyond it q is zero in fp32; min.NaN passes a NaN on.
+// t P(t) e with t = 1 / (1 + 0.28 a), P with six coefficients of our own fit instead of five (largest error of the
+// coefficients as they stand 1.1e-8, at a = 1.09; roundings make it 2e-7 at a = 0, where the sum to 0.5 counts).  erff and
+// expf took 33 instructions an element and twice the time of the bytes in bf16; this takes a reciprocal, an exponential and
+// the rest in packed pairs.  15: beyond it q is zero in fp32; min.NaN passes a NaN on.
+//
+// fp32 takes another form of q where a < 1: there q is of the order of one half, and its absolute error shows (x Phi(x) off by
+// 4.7e-7 relative, erff's form by 2.1e-7; with this 2.7e-7; from 1 on 8e-8 absolute on the negative side, erff's form
+// 1.2e-7).  q = a P(a^2) - 1/2, P a polynomial of our own fit, with the coefficients rounded off by 8e-8 relative to q at 1.  The
+// one that counts is taken by products, not by selects, whose pipe is the busier one: the weight 2^25 (1 - a), saturated,
+// is exactly 1 below a = 1 and 0 from there on, and the difference of two such close numbers is exact.  12608x4096, with
+// dropout: forward 61.6 -> 65.7 us, backward 89.9 -> 89.3, and 61.6 without (erff and expf: 87 and 115, 68 without).
+template <typename T>
 __device__ __forceinline__ void normal_tail(float2 x, float2& a, float2& q, float2& e) {
     float u, v;
     split2(x, u, v);
@@ -46,11 +54,22 @@ __device__ __forceinline__ void normal_tail(float2 x, float2& a, float2& q, floa
     s = fma2(s, t, splat2(-0.0674976185f));
     s = fma2(s, t, splat2(-0.116520643f));
     q = mul2(mul2(s, t), e);
+    if constexpr (sizeof(T) == 4) {
+        s = mul2(a, a);
+        float2 p = fma2(splat2(-7.462909252353711e-06f), s, splat2(0.0001129522206611f));
+        p = fma2(p, s, splat2(-0.0011857850477099419f));
+        p = fma2(p, s, splat2(0.009973078034818172f));
+        p = fma2(p, s, splat2(-0.06649031490087509f));
+        p = fma2(p, s, splat2(0.3989422917366028f));
+        split2(fma2(a, splat2(-33554432.f), splat2(33554432.f)), u, v);
+        q = fma2(make_float2(__saturatef(u), __saturatef(v)), add2(fma2(a, p, splat2(-0.5f)), mul2(q, splat2(-1.f))), q);
+    }
 }
 // x Phi(x) = max(x, 0) + |x| q: zero at minus infinity, its limit
+template <typename T>
 __device__ __forceinline__ float2 gelu2(float2 x) {
     float2 a, q, e;
-    normal_tail(x, a, q, e);
+    normal_tail<T>(x, a, q, e);
     float u, v;
     split2(x, u, v);
     return fma2(a, q, make_float2(fmaxf(u, 0.f), fmaxf(v, 0.f)));
@@ -58,22 +77,32 @@ __device__ __forceinline__ float2 gelu2(float2 x) {
 __device__ __forceinline__ float flip(float u, float sign) {
     return __uint_as_float(__float_as_uint(u) ^ (__float_as_uint(sign) & 0x80000000u));
 }
-// Phi(x) + x phi(x) = 1/2 + sign(x) (1/2 + q + a phi(a))
+// Phi(x) + x phi(x).  16-bit types: 1/2 + sign(x) (1/2 + q + a phi(a)).  fp32: q + a phi(a) with the sign of x, and one more for
+// a positive x, so that the negative side keeps its digits.
+template <typename T>
 __device__ __forceinline__ float2 gelu_slope2(float2 x) {
     float2 a, q, e;
-    normal_tail(x, a, q, e);
+    normal_tail<T>(x, a, q, e);
+    const float2 c = splat2(0.39894228040143268f);
     float u, v, xu, xv;
-    split2(add2(fma2(mul2(a, splat2(0.39894228040143268f)), e, splat2(0.5f)), q), u, v);
     split2(x, xu, xv);
-    return add2(make_float2(flip(u, xu), flip(v, xv)), splat2(0.5f));
+    if constexpr (sizeof(T) == 2) {
+        split2(add2(fma2(mul2(a, c), e, splat2(0.5f)), q), u, v);
+        return add2(make_float2(flip(u, xu), flip(v, xv)), splat2(0.5f));
+    } else {
+        split2(fma2(mul2(a, c), e, q), u, v);
+        // by the sign bit: minus zero goes with the negative side
+        return add2(make_float2(flip(u, xu), flip(v, xv)),
+                    make_float2(__float_as_int(xu) < 0 ? 0.f : 1.f, __float_as_int(xv) < 0 ? 0.f : 1.f));
+    }
 }
 
-template <int OP, int N>
+template <typename T, int OP, int N>
 __device__ __forceinline__ void point_apply(float2 (&x)[N], const float2 (&o)[N], bool has_other, const DropArgs& d,
                                             unsigned long long start) {
     if constexpr (OP != POINT_DROPOUT) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = OP == POINT_GELU ? gelu2(x[j]) : mul2(o[j], gelu_slope2(x[j]));
+        for (int j = 0; j < N; ++j) x[j] = OP == POINT_GELU ? gelu2<T>(x[j]) : mul2(o[j], gelu_slope2<T>(x[j]));
     }
     // in the backward the mask comes last: what the forward dropped gets a zero whatever its x was
     if (d.on) mam_drop_pairs<N>(x, start, false, d.threshold, d.scale);
@@ -84,6 +113,10 @@ __device__ __forceinline__ void point_apply(float2 (&x)[N], const float2 (&o)[N]
 }
 
 constexpr int POINT_THREADS = 128;
+// CTAs on an SM: the forward of GELU in fp32 needs 40 registers, and twelve CTAs take 67.7 us where eight or ten take 69.8
+// (12608x4096 with dropout)
+template <typename T, int OP, int MODE>
+constexpr int POINT_CTAS = sizeof(T) == 4 && OP == POINT_GELU && MODE == ALIGNED ? 12 : 8;
 
 // NV vectors a thread, all loads first; a CTA a block (CTAs that walk over several blocks took a sixth fewer instructions and
 // a tenth longer: their loads wait for the stores before them).  ALIGNED: whole vectors only, n is a multiple of them; with TAIL
@@ -91,7 +124,7 @@ constexpr int POINT_THREADS = 128;
 // others a tenth).
 // RAGGED: any n and any alignment, with the loads and stores of ragged rows, the whole tensor being one row.
 template <typename T, int NV, int OP, int MODE, bool TAIL>
-__global__ void __launch_bounds__(POINT_THREADS, 8) mam_point_kernel(const __grid_constant__ PointParams p) {
+__global__ void __launch_bounds__(POINT_THREADS, POINT_CTAS<T, OP, MODE>) mam_point_kernel(const __grid_constant__ PointParams p) {
     constexpr int V = VEC<T>;
     const bool has = p.other != nullptr;
     const RowSrc<T, MODE> x(static_cast<const T*>(p.x), 0, 1, p.n, static_cast<const T*>(p.x)),
@@ -112,7 +145,7 @@ __global__ void __launch_bounds__(POINT_THREADS, 8) mam_point_kernel(const __gri
                 const bool two = e + 1 < p.tail;
                 float2 f[1] = {make_float2(to_f32(xt[e]), two ? to_f32(xt[e + 1]) : 0.f)}, g[1] = {splat2(0.f)};
                 if (has) g[0] = make_float2(to_f32(ot[e]), two ? to_f32(ot[e + 1]) : 0.f);
-                point_apply<OP>(f, g, has, p.drop, mam_drop_start(seed, p.n + e));
+                point_apply<T, OP>(f, g, has, p.drop, mam_drop_start(seed, p.n + e));
                 out[p.n + e] = from_f32<T>(f[0].x);
                 if (two) out[p.n + e + 1] = from_f32<T>(f[0].y);
             }
@@ -138,7 +171,7 @@ __global__ void __launch_bounds__(POINT_THREADS, 8) mam_point_kernel(const __gri
             float2 f[V / 2], g[V / 2];
             unpack<T>(px[i], f);
             if (has) unpack<T>(po[i], g);
-            point_apply<OP>(f, g, has, p.drop, start + (unsigned long long)(i * (STEP / 2)) * MAM_DROP_STEP);
+            point_apply<T, OP>(f, g, has, p.drop, start + (unsigned long long)(i * (STEP / 2)) * MAM_DROP_STEP);
             q = pack<T>(f);
         }
         const int rest = MODE == RAGGED ? (int)max(min(p.n - at, 2LL * V), 0LL) : at < p.n ? V : 0;

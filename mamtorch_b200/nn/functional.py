@@ -501,5 +501,6 @@ def dropout(x: Tensor, drop_rate: float, drop_seed=None, residual: Tensor | None
 
 
 def gelu(x: Tensor, drop_rate: float = 0.0, drop_seed=None) -> Tensor:
-    """dropout(x * Phi(x)), Phi the integral of the normal distribution: the exact GELU, with the dropout behind it."""
+    """dropout(x * Phi(x)), Phi the integral of the normal distribution: the exact GELU, with the dropout behind it.  At minus
+    infinity the value is 0, its limit (torch's is NaN)."""
     return (_C.gelu if _eager(x) else _ops.gelu.default)(x, *_drop_args(drop_rate, drop_seed))

@@ -1,6 +1,7 @@
-"""Layer norm, dropout and GELU operators: first calls of a process, copies of modules, waits that run out, what GELU's form is worth
-in fp32."""
+"""Layer norm, dropout and GELU operators: first calls of a process, copies of modules, waits that run out, what GELU's form is
+worth."""
 import copy
+import math
 import os
 import subprocess
 import sys
@@ -234,3 +235,42 @@ def test_the_first_call_of_a_process_inside_a_capture(cuda):
             print("same")
         """, backward)
         assert out.strip() == "same"
+
+
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1 << 22, (1 << 21) + 1])
+def test_gelu_over_a_dense_grid(cuda, n, t):
+    """The elementwise error of GELU and its slope on [-15, 15], in eps = 2^-24, half a step of fp32.
+
+    fp32, |x| < 1: Phi(-a) = 1/2 - a P, a = |x|.  P's roundings are 1.36 eps of P (its last step one, the step before and a^2 damped
+    by the coefficients), a P / Phi(-a) is 2.15 at most, the coefficients are off by 1.4 eps relative to Phi(-a), it rounds once,
+    and so does its product with a: 2.15 * 1.36 + 1.4 + 2 = 6.4 eps relative.  The slope's a P - 1/2 + a c e: 1.36 eps a P + eps / 4,
+    a c e within 1.5 eps (e = ex2, two units in the last place, its argument twice rounded, times 0.242; a c), the sum eps / 4, and
+    one more added, eps: 3.5 eps.
+    Elsewhere, and in 16-bit types everywhere, Phi(-a) = s(t) t e: t within 3 eps (sum, reciprocal), each step of s one eps of its
+    value, e as above, two products, the fit 1.1e-8: a Phi(-a) within 3.2 eps for a >= 1 and 3.4 for all a, the slope's sum
+    within 4.8 eps for a >= 1, and 12 for all a, where 1/2 is added twice to sums of the order of one.  Then one rounding to
+    fp32 relative to the value, one to t, and the product with the upstream gradient, which is one."""
+    from mamtorch_b200.nn import functional as MF
+
+    eps, half = 2.0 ** -24, torch.finfo(t).eps / 2
+    x = torch.linspace(-15, 15, n, device=cuda, dtype=torch.float64).to(t).requires_grad_()
+    y = MF.gelu(x)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    z = x.detach().double()
+    phi = 0.5 * torch.erfc(-z / math.sqrt(2))
+    want, slope = z * phi, phi + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    near = (z.abs() < 1) & (t == torch.float32)
+    far_y, far_slope = (3.2, 4.8) if t == torch.float32 else (3.4, 12.0)
+    rounded = 0.0 if t == torch.float32 else half
+    bound = torch.where(near, 6.4 * eps * want.abs(), far_y * eps + eps * want.abs()) + rounded * want.abs() + tiny
+    assert ((y.detach().double() - want).abs() - bound).max().item() <= 0
+    bound = torch.where(near, 3.5 * eps, far_slope * eps + eps * slope.abs()) + rounded * slope.abs() + tiny
+    assert ((dx.double() - slope).abs() - bound).max().item() <= 0
+    if t == torch.float32:      # no less exact than the erff form that it stands for: 10 % for the grid's luck
+        other = torch.nn.functional.gelu(x.detach()).double()
+        middle = near & (z != 0)
+        rms = lambda v: ((v - want)[middle] / want[middle]).square().mean().sqrt().item()   # noqa: E731
+        assert rms(y.detach().double()) <= 1.1 * rms(other)
+        assert (y.detach().double() - want).abs().max() <= (other - want).abs().max()
