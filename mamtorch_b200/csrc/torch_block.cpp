@@ -226,9 +226,19 @@ Tensor gelu_backward(const Tensor& gy, const Tensor& x, double rate, int64_t see
 // ---------------------------------------------------------------- differentiable operators
 
 // The operators above through the dispatcher, so that tracing with fake tensors reaches their shape functions.
+// A seed is a number that may be symbolic: a compiled graph takes it as an argument instead of being compiled for each.
+template <class A>
+using Symbolic = std::conditional_t<std::is_same_v<A, int64_t>, c10::SymInt, A>;
+template <class Fn>
+struct SymbolicFn;
+template <class R, class... A>
+struct SymbolicFn<R(A...)> {
+    using type = R(Symbolic<A>...);
+};
 #define MAM_OP(name, fn)                                                                                          \
-    static const auto name =                                                                                      \
-        c10::Dispatcher::singleton().findSchemaOrThrow("mamtorch_b200::" #fn, "").typed<decltype(fn)>()
+    static const auto name = c10::Dispatcher::singleton()                                                         \
+                                 .findSchemaOrThrow("mamtorch_b200::" #fn, "")                                    \
+                                 .typed<SymbolicFn<decltype(fn)>::type>()
 
 template <class... Ts>
 bool wants_grad(const Ts&... ts) {
@@ -261,8 +271,8 @@ template <class Fn, const char* NAME>
 struct Inner;
 template <class R, class... A, const char* NAME>
 struct Inner<R(A...), NAME> {
-    static R call(A... args) {
-        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<R(A...)>();
+    static R call(Symbolic<A>... args) {
+        static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<R(Symbolic<A>...)>();
         refuse_tangents(tensor_of(args)...);
         std::shared_ptr<torch::autograd::Error> node;
         if (wants_grad(tensor_of(args)...))
@@ -282,12 +292,12 @@ struct Inner<R(A...), NAME> {
 // took as long as an allocation.
 struct BlockNode : torch::autograd::Node {
     double rate = 0;
-    int64_t seed = 0;
+    c10::SymInt seed = 0;
     SavedVariable seed_at;
     void release_variables() override { seed_at.reset_data(); }
 };
 template <class N, class... Ts>
-std::shared_ptr<N> make_node(double rate, int64_t seed, const OptTensor& seed_at, const Ts&... inputs) {
+std::shared_ptr<N> make_node(double rate, c10::SymInt seed, const OptTensor& seed_at, const Ts&... inputs) {
     std::shared_ptr<N> n(new N(), torch::autograd::deleteNode);
     n->rate = rate;
     n->seed = seed;
@@ -364,7 +374,7 @@ struct GeluBackward : BlockNode {       // input: x
 // below the autograd keys, so that the levels further out differentiate it too.  (The norm's node needs the statistics
 // and calls the inner operator: what a level further out would differentiate then is refused there.)
 std::vector<Tensor> norm_node(const Tensor& x, const Tensor& res, const Tensor& w, const Tensor& b, double eps, double rate,
-                              int64_t seed, const OptTensor& seed_at) {
+                              c10::SymInt seed, const OptTensor& seed_at) {
     MAM_OP(op, layer_norm_forward);
     auto node = make_node<NormBackward>(rate, seed, seed_at, x, res, w, b);
     std::vector<Tensor> out;
@@ -383,7 +393,7 @@ std::vector<Tensor> norm_node(const Tensor& x, const Tensor& res, const Tensor& 
     return out;
 }
 std::vector<Tensor> norm_plain(const Tensor& x, const OptTensor& residual, const OptTensor& weight, const OptTensor& bias,
-                               double eps, double rate, int64_t seed, const OptTensor& seed_at) {
+                               double eps, double rate, c10::SymInt seed, const OptTensor& seed_at) {
     MAM_OP(op, layer_norm_forward);
     return op.call(x, residual, weight, bias, eps, rate, seed, seed_at, false);
 }
@@ -399,7 +409,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
     return std::move(norm_plain(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt)[0]);
 }
 std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
-                                                  const OptTensor& bias, double eps, double rate, int64_t seed,
+                                                  const OptTensor& bias, double eps, double rate, c10::SymInt seed,
                                                   const OptTensor& seed_at) {
     const Tensor w = plain(weight), b = plain(bias);
     refuse_tangents(x, residual, w, b);
@@ -416,7 +426,7 @@ std::tuple<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor&
     }
     return {std::move(out[0]), std::move(out[1])};
 }
-Tensor dropout(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
+Tensor dropout(const Tensor& x, const OptTensor& residual, double rate, c10::SymInt seed, const OptTensor& seed_at) {
     MAM_OP(op, dropout_forward);
     MAM_OP(self, dropout);
     const Tensor res = plain(residual);
@@ -430,7 +440,7 @@ Tensor dropout(const Tensor& x, const OptTensor& residual, double rate, int64_t 
     if (node) torch::autograd::set_history(y, node);
     return y;
 }
-Tensor gelu(const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
+Tensor gelu(const Tensor& x, double rate, c10::SymInt seed, const OptTensor& seed_at) {
     MAM_OP(op, gelu_forward);
     MAM_OP(self, gelu);
     refuse_tangents(x);
@@ -452,16 +462,16 @@ Tensor layer_norm_below(const Tensor& x, const OptTensor& weight, const OptTenso
     return std::move(norm_plain(x, std::nullopt, weight, bias, eps, 0.0, 0, std::nullopt)[0]);
 }
 std::tuple<Tensor, Tensor> dropout_add_layer_norm_below(const Tensor& x, const Tensor& residual, const OptTensor& weight,
-                                                        const OptTensor& bias, double eps, double rate, int64_t seed,
+                                                        const OptTensor& bias, double eps, double rate, c10::SymInt seed,
                                                         const OptTensor& seed_at) {
     auto out = norm_plain(x, residual, weight, bias, eps, rate, seed, seed_at);
     return {std::move(out[0]), std::move(out[1])};
 }
-Tensor dropout_below(const Tensor& x, const OptTensor& residual, double rate, int64_t seed, const OptTensor& seed_at) {
+Tensor dropout_below(const Tensor& x, const OptTensor& residual, double rate, c10::SymInt seed, const OptTensor& seed_at) {
     MAM_OP(op, dropout_forward);
     return op.call(x, residual, rate, seed, seed_at);
 }
-Tensor gelu_below(const Tensor& x, double rate, int64_t seed, const OptTensor& seed_at) {
+Tensor gelu_below(const Tensor& x, double rate, c10::SymInt seed, const OptTensor& seed_at) {
     MAM_OP(op, gelu_forward);
     return op.call(x, rate, seed, seed_at);
 }
@@ -469,10 +479,12 @@ Tensor gelu_below(const Tensor& x, double rate, int64_t seed, const OptTensor& s
 // Eager calls from Python: straight to the functions above, under a transform by way of the dispatcher.
 template <class Fn, const char* NAME>
 struct Eager;
+template <class A>
+using Plain = std::conditional_t<std::is_same_v<A, c10::SymInt>, int64_t, A>;
 template <class R, class... A, const char* NAME>
 struct Eager<R(A...), NAME> {
     template <R (*FN)(A...)>
-    static R call(A... args) {
+    static R call(Plain<A>... args) {
         if (!transformed()) return FN(args...);
         static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(NAME, "").typed<R(A...)>();
         return op.call(args...);
@@ -488,15 +500,15 @@ constexpr char kNormForward[] = "mamtorch_b200::layer_norm_forward", kNormBackwa
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(mamtorch_b200, m) {
-    m.def("layer_norm_forward(Tensor x, Tensor? residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, int drop_seed, Tensor? drop_seed_at, bool want_stats) -> Tensor[]");
-    m.def("layer_norm_backward(Tensor? gy, Tensor? gsum, Tensor s, Tensor stats, Tensor? weight, float drop_rate, int drop_seed, Tensor? drop_seed_at, bool params_f32, bool want_weight, bool want_bias) -> Tensor[]");
-    m.def("dropout_forward(Tensor x, Tensor? residual, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
-    m.def("gelu_forward(Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
-    m.def("gelu_backward(Tensor gy, Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("layer_norm_forward(Tensor x, Tensor? residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at, bool want_stats) -> Tensor[]");
+    m.def("layer_norm_backward(Tensor? gy, Tensor? gsum, Tensor s, Tensor stats, Tensor? weight, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at, bool params_f32, bool want_weight, bool want_bias) -> Tensor[]");
+    m.def("dropout_forward(Tensor x, Tensor? residual, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("gelu_forward(Tensor x, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("gelu_backward(Tensor gy, Tensor x, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at) -> Tensor");
     m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps) -> Tensor");
-    m.def("dropout_add_layer_norm(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> (Tensor, Tensor)");
-    m.def("dropout(Tensor x, Tensor? residual, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
-    m.def("gelu(Tensor x, float drop_rate, int drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("dropout_add_layer_norm(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at) -> (Tensor, Tensor)");
+    m.def("dropout(Tensor x, Tensor? residual, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at) -> Tensor");
+    m.def("gelu(Tensor x, float drop_rate, SymInt drop_seed, Tensor? drop_seed_at) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(mamtorch_b200, CUDA, m) {
     m.impl("layer_norm_forward", &layer_norm_forward);

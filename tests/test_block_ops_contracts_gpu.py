@@ -274,3 +274,28 @@ def test_gelu_over_a_dense_grid(cuda, n, t):
         rms = lambda v: ((v - want)[middle] / want[middle]).square().mean().sqrt().item()   # noqa: E731
         assert rms(y.detach().double()) <= 1.1 * rms(other)
         assert (y.detach().double() - want).abs().max() <= (other - want).abs().max()
+
+
+def test_compiled_calls_take_any_seed(cuda):
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    from mamtorch_b200.nn import functional as MF
+
+    w, b = torch.randn(72, device=cuda), torch.randn(72, device=cuda)
+    gy = torch.randn(40, 72, device=cuda)
+
+    def step(x, seed):
+        y, s = MF.dropout_add_layer_norm(MF.gelu(x, 0.25, seed), x, w, b, 1e-5, 0.5, seed + 1)
+        return MF.dropout(y, 0.5, seed + 2, residual=s)
+
+    torch._dynamo.reset()
+    counter = CompileCounterWithBackend("aot_eager")
+    compiled = torch.compile(step, backend=counter, fullgraph=True)
+    for seed in (3, 4, 2 ** 61 + 5, 7, 11, 2 ** 62 - 9, 12, 13, 14, 15, 16, 17):
+        x = torch.randn(40, 72, device=cuda, requires_grad=True)
+        got, want = compiled(x, seed), step(x, seed)
+        assert torch.equal(got, want)
+        # the same kernels on the same numbers; autograd may add x's three gradients in another order
+        torch.testing.assert_close(torch.autograd.grad(got, x, gy), torch.autograd.grad(want, x, gy), rtol=1e-5, atol=1e-5)
+    assert counter.frame_count <= 2
+    torch._dynamo.reset()

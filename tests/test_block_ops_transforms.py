@@ -217,3 +217,39 @@ def test_vmap_over_seeds_gives_each_sample_its_mask():
         lib.impl("dropout_forward", lambda x, res, rate, seed, at: drop(x, rate, seed + int(at)), "CPU")
         got = torch.func.vmap(lambda s: MF.dropout(x, 0.5, s))(seeds)
     assert torch.equal(got, torch.stack([drop(x, 0.5, int(s)) for s in seeds]))
+
+
+# ---------------------------------------------------------------- torch.compile
+
+def test_compiled_calls_take_any_seed(cpu_kernels):
+    """A seed is an argument of the compiled graph, not a constant of it: one graph for the first, one for all others."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    def step(x, seed):
+        y, s = MF.dropout_add_layer_norm(MF.gelu(x, 0.25, seed), x, W, B, 1e-5, 0.5, seed + 1)
+        return MF.dropout(y, 0.5, seed + 2, residual=s)
+
+    torch._dynamo.reset()
+    counter = CompileCounterWithBackend("aot_eager")
+    compiled = torch.compile(step, backend=counter, fullgraph=True)
+    for seed in (3, 4, 2 ** 61 + 5, 7, 11, 2 ** 62 - 9, 10 ** 9, 12, 13, 14, 15, 16):
+        x, z = X.clone().requires_grad_(), X.clone().requires_grad_()
+        got, want = compiled(x, seed), step(z, seed)
+        assert torch.equal(got, want)
+        torch.testing.assert_close(torch.autograd.grad(got, x, V), torch.autograd.grad(want, z, V), **CLOSE)
+    assert counter.frame_count <= 2
+    torch._dynamo.reset()
+
+
+def test_seeds_are_whole_64_bit_numbers(cpu_kernels):
+    seen = []
+    with torch.library._scoped_library("mamtorch_b200", "IMPL") as lib:
+        lib.impl("dropout_forward", lambda x, res, rate, seed, at: seen.append(seed) or x.clone(), "CPU", allow_override=True)
+        seeds = (0, -1, 2 ** 63 - 1, -2 ** 63, -2 ** 62 - 7, 2 ** 62 + 1)
+        for seed in seeds:
+            x = X.clone().requires_grad_()
+            torch.autograd.grad(MF.dropout(x, 0.5, seed), x, V)
+    assert [int(s) for s in seen] == [s for s in seeds for _ in range(2)]
+    for seed in (2 ** 63, -2 ** 63 - 1):
+        with pytest.raises((TypeError, RuntimeError, OverflowError)):
+            MF.dropout(X, 0.5, seed)
