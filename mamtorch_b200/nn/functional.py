@@ -461,17 +461,23 @@ def _eager(x) -> bool:
     return not (torch.compiler.is_compiling() or torch.overrides.has_torch_function_unary(x))
 
 
-def _drop_args(rate: float, seed):
+def _draw_seed(on_cuda: bool) -> int:
+    if on_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a number drawn during a graph capture would repeat one mask at every replay: "
+                           "pass drop_seed, as a tensor for a mask of its own at each replay")
+    return fresh_drop_seed()
+
+
+def _drop_args(x: Tensor, rate: float, seed):
     rate = float(rate)
     if not 0.0 <= rate < 1.0:
         raise ValueError(f"drop_rate must be in [0, 1), not {rate}")
     if rate == 0.0:
         return 0.0, 0, None
     if seed is None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a number drawn during a graph capture would repeat one mask at every replay: "
-                               "pass drop_seed, as a tensor for a mask of its own at each replay")
-        return rate, fresh_drop_seed(), None
+        # never traced: a compiled graph would hold the answer of its first call
+        draw = torch._disable_dynamo(_draw_seed) if torch.compiler.is_compiling() else _draw_seed
+        return rate, draw(x.is_cuda), None
     if isinstance(seed, Tensor):
         return rate, 0, seed
     return rate, int(seed), None
@@ -489,7 +495,7 @@ def dropout_add_layer_norm(x: Tensor, residual: Tensor, weight: Tensor | None = 
     One pass forward and one backward; equal to `dropout(x, ..., residual)` followed by `layer_norm`, which reads s as it
     is stored: s bit for bit, y up to the order of a row's fp32 sums."""
     f = _C.dropout_add_layer_norm if _eager(x) else _ops.dropout_add_layer_norm.default
-    return f(x, residual, weight, bias, eps, *_drop_args(drop_rate, drop_seed))
+    return f(x, residual, weight, bias, eps, *_drop_args(x, drop_rate, drop_seed))
 
 
 def dropout(x: Tensor, drop_rate: float, drop_seed=None, residual: Tensor | None = None) -> Tensor:
@@ -497,10 +503,10 @@ def dropout(x: Tensor, drop_rate: float, drop_seed=None, residual: Tensor | None
     always drops (a training-time operator), and is refused under vmap, where one seed would give all samples one mask, unless
     the seeds are mapped over too.  Its masks are not those of `weight_drop` and the MAM layers' output dropout:
     it takes one 64-bit draw for two elements, they take one for each."""
-    return (_C.dropout if _eager(x) else _ops.dropout.default)(x, residual, *_drop_args(drop_rate, drop_seed))
+    return (_C.dropout if _eager(x) else _ops.dropout.default)(x, residual, *_drop_args(x, drop_rate, drop_seed))
 
 
 def gelu(x: Tensor, drop_rate: float = 0.0, drop_seed=None) -> Tensor:
     """dropout(x * Phi(x)), Phi the integral of the normal distribution: the exact GELU, with the dropout behind it.  At minus
     infinity the value is 0, its limit (torch's is NaN)."""
-    return (_C.gelu if _eager(x) else _ops.gelu.default)(x, *_drop_args(drop_rate, drop_seed))
+    return (_C.gelu if _eager(x) else _ops.gelu.default)(x, *_drop_args(x, drop_rate, drop_seed))

@@ -298,4 +298,11 @@ def test_compiled_calls_take_any_seed(cuda):
         # the same kernels on the same numbers; autograd may add x's three gradients in another order
         torch.testing.assert_close(torch.autograd.grad(got, x, gy), torch.autograd.grad(want, x, gy), rtol=1e-5, atol=1e-5)
     assert counter.frame_count <= 2
+    # a drawn seed: a new one at each call, and none inside a capture, however the call was compiled
+    drawn = torch.compile(lambda v: MF.dropout(v, 0.5), backend="aot_eager")
+    x = torch.ones(4096, device=cuda)
+    assert not torch.equal(drawn(x), drawn(x))
+    with pytest.raises(RuntimeError, match="capture"), pytest.warns(UserWarning, match="empty"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            drawn(x)
     torch._dynamo.reset()

@@ -241,6 +241,23 @@ def test_compiled_calls_take_any_seed(cpu_kernels):
     torch._dynamo.reset()
 
 
+def test_compiled_calls_that_draw_their_seeds(cpu_kernels):
+    """The draw from torch's CPU generator breaks the graph; what follows it is compiled once more, not for each number."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    torch._dynamo.reset()
+    counter = CompileCounterWithBackend("aot_eager")
+    step = lambda x: MF.gelu(MF.dropout(x, 0.5) * 2)     # noqa: E731
+    compiled = torch.compile(step, backend=counter)
+    for k in range(12):
+        torch.manual_seed(k)
+        got = compiled(X)
+        torch.manual_seed(k)
+        assert torch.equal(got, step(X))
+    assert counter.frame_count <= 4
+    torch._dynamo.reset()
+
+
 def test_seeds_are_whole_64_bit_numbers(cpu_kernels):
     seen = []
     with torch.library._scoped_library("mamtorch_b200", "IMPL") as lib:
@@ -253,3 +270,9 @@ def test_seeds_are_whole_64_bit_numbers(cpu_kernels):
     for seed in (2 ** 63, -2 ** 63 - 1):
         with pytest.raises((TypeError, RuntimeError, OverflowError)):
             MF.dropout(X, 0.5, seed)
+
+
+def test_a_seed_drawn_for_a_cpu_tensor_asks_no_driver():
+    for f in (lambda: MF.dropout(X, 0.5), lambda: MF.gelu(X, 0.5), lambda: MF.dropout_add_layer_norm(X, X, drop_rate=0.5)):
+        with pytest.raises(NotImplementedError):
+            f()
