@@ -475,9 +475,7 @@ def _drop_args(x: Tensor, rate: float, seed):
     if rate == 0.0:
         return 0.0, 0, None
     if seed is None:
-        # never traced: a compiled graph would hold the answer of its first call
-        draw = torch._disable_dynamo(_draw_seed) if torch.compiler.is_compiling() else _draw_seed
-        return rate, draw(x.is_cuda), None
+        return rate, _draw_seed(x.is_cuda), None
     if isinstance(seed, Tensor):
         return rate, 0, seed
     return rate, int(seed), None

@@ -306,3 +306,31 @@ def test_compiled_calls_take_any_seed(cuda):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             drawn(x)
     torch._dynamo.reset()
+
+
+def test_a_compiled_module_in_a_captured_graph_drops_anew_at_each_replay(cuda):
+    """Compiled outside of a capture first: that answer must not stay."""
+    from mamtorch_b200.nn.vit import MAMMlpBlock
+
+    torch._dynamo.reset()
+    torch.manual_seed(0)
+    block = MAMMlpBlock(64, 128, fused=True, drop_rate=0.5).to(cuda)
+    compiled = torch.compile(block, backend="aot_eager")
+    x = torch.randn(40, 64, device=cuda)
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(3):
+                compiled(x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert not torch.equal(compiled(x), compiled(x))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = compiled(x)
+        outs = []
+        for _ in range(3):
+            graph.replay()
+            outs.append(y.clone())
+    assert not torch.equal(outs[0], outs[1]) and not torch.equal(outs[1], outs[2])
+    torch._dynamo.reset()
