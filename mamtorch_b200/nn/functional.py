@@ -194,16 +194,17 @@ def _(gy, x, drop_rate, drop_seed, drop_seed_at):
     return x.new_empty(x.shape)
 
 
-def _register_vmap(name):
-    """Under vmap the operators run sample by sample.  With one seed for all samples each would lose the same elements, since
-    a mask is a function of the seed and the element's number within its sample: refused."""
+def _register_vmap(name, forward):
+    """Under vmap the operators run sample by sample.  A forward with one seed for all samples would lose the same elements in
+    each, since a mask is a function of the seed and the element's number within its sample: refused.  A backward that is
+    mapped has one forward behind all its gradients, and that one's mask."""
     op = getattr(_ops, name).default
     names = [a.name for a in op._schema.arguments]
     rate, seed_at = (names.index(n) if n in names else None for n in ("drop_rate", "drop_seed_at"))
 
     @torch.library.register_vmap(f"mamtorch_b200::{name}")
     def _(info, in_dims, *args):
-        if rate is not None and args[rate] > 0 and in_dims[seed_at] is None:
+        if forward and rate is not None and args[rate] > 0 and in_dims[seed_at] is None:
             raise RuntimeError(f"mamtorch_b200::{name} under vmap would drop the same elements in every sample: call it on the "
                                "whole batch, or map over a tensor of seeds too")
         outs = [op(*(a if d is None else a.select(d, i) for a, d in zip(args, in_dims))) for i in range(info.batch_size)]
@@ -213,9 +214,10 @@ def _register_vmap(name):
         return kind(torch.stack(o) for o in zip(*outs)), kind(0 for _ in outs[0])
 
 
-for _op_name in ("layer_norm", "dropout_add_layer_norm", "dropout", "gelu", "layer_norm_forward", "layer_norm_backward",
-              "dropout_forward", "gelu_forward", "gelu_backward"):
-    _register_vmap(_op_name)
+for _op_name in ("layer_norm", "dropout_add_layer_norm", "dropout", "gelu", "layer_norm_forward", "gelu_forward"):
+    _register_vmap(_op_name, True)
+for _op_name in ("layer_norm_backward", "gelu_backward", "dropout_forward"):     # the last is the dropout's backward too
+    _register_vmap(_op_name, False)
 
 
 @torch.library.register_fake("mamtorch_b200::dense_nt")

@@ -189,8 +189,16 @@ def test_vmap_of_a_dropout_is_refused(cpu_kernels, name):
               lambda v: torch.func.vjp(f, v)[1](V)[0]):
         with pytest.raises(RuntimeError, match="same elements in every sample"):
             torch.func.vmap(g)(xs)
-    with pytest.raises(RuntimeError, match="same elements in every sample"):
-        torch.func.vmap(lambda g: torch.ops.mamtorch_b200.dropout_forward(g, None, 0.5, 3, None))(xs)
+
+
+@pytest.mark.parametrize("name", OPS)
+def test_many_upstream_gradients_of_one_call(cpu_kernels, name):
+    """Mapped over the gradients alone: the forward is one, and so is its mask."""
+    f, plain = OPS[name]
+    want = torch.func.jacrev(plain)(X)
+    torch.testing.assert_close(torch.func.jacrev(f)(X), want, **CLOSE)
+    torch.testing.assert_close(torch.func.vmap(torch.func.vjp(f, X)[1])(torch.eye(18, dtype=F64).view(18, 3, 6))[0].view_as(want), want,
+                               **CLOSE)
 
 
 def test_vmap_without_a_dropout_goes_sample_by_sample(cpu_kernels):
