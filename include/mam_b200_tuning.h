@@ -21,8 +21,8 @@ enum mam_tune_knob {
                                   3 / 4 one row of dX per warp (a parked in shared memory / read through L1)  */
     MAM_TUNE_DENSE_SPLIT = 4,  /* TF32 product: 1 slices the tiles of the last partial wave (default), 0 not  */
     MAM_TUNE_CONV_DIRECT_ROWS = 5, /* output rows per CTA of the one-kernel convolution backward, 0 by size   */
-    MAM_TUNE_NORM_WAIT = 6     /* polls after which a layer norm's wait for a row in shared memory gives up:
-                                  -1 the library's own limit (default), 0 at once                            */
+    MAM_TUNE_NORM_LATE = 6     /* 1: the first wait of a layer norm's threads for a row in shared memory counts
+                                  as run out, 0: it does not (default)                                       */
 };
 
 /* Sets one knob; MAM_ERR_INVALID_ARGUMENT for an unknown knob or a value outside its range. */

@@ -32,7 +32,6 @@ int drop_args(float rate, uint64_t seed, const int64_t* seed_at, DropArgs* d) {
 }
 
 // ---- rows through shared memory ----
-constexpr unsigned RING_POLLS = 1u << 22;      // of a wait for a row; each may suspend the thread for a while
 // A row of the ring in shared memory; ragged ones have up to 15 bytes in front, and are read 16 bytes beyond their end.
 size_t ring_slot(int64_t width, int size, bool aligned) {
     return aligned ? (size_t)width * size : ((size_t)width * size + 15) / 16 * 16 + 32;
@@ -76,7 +75,7 @@ NormRing ring_of(int64_t width, int group, int groups, int stages, int size, int
     r.weights_at = (unsigned)(((size_t)tensors * r.slot_bytes * groups * stages + 127) / 128 * 128);
     r.bars_at = (unsigned)(r.weights_at + params * ((width + 7) / 8 * 8 * 4));
     r.bytes = r.bars_at + groups * stages * 8;
-    r.polls = g_norm_wait < 0 ? RING_POLLS : (unsigned)g_norm_wait;
+    r.late = g_norm_late;
     return r;
 }
 

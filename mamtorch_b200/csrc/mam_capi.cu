@@ -686,9 +686,9 @@ int mam_tune_set(int knob, int value) {
             if (value < 0 || value > 64) return MAM_ERR_INVALID_ARGUMENT;
             g_conv_direct_rows = value;
             return MAM_OK;
-        case MAM_TUNE_NORM_WAIT:
-            if (value < -1) return MAM_ERR_INVALID_ARGUMENT;
-            g_norm_wait = value;
+        case MAM_TUNE_NORM_LATE:
+            if (value < 0 || value > 1) return MAM_ERR_INVALID_ARGUMENT;
+            g_norm_late = value;
             return MAM_OK;
         default:
             return MAM_ERR_INVALID_ARGUMENT;

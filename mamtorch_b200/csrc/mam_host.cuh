@@ -48,7 +48,7 @@ inline int device_info(const DevInfo** out) {
     return d.major == 10 ? MAM_OK : MAM_ERR_NOT_SM100;
 }
 
-inline int g_norm_wait = -1;  // polls of the norm's ring (MAM_TUNE_NORM_WAIT), or -1: the constant
+inline int g_norm_late = 0;   // 1: the first wait of the norm's ring counts as run out (MAM_TUNE_NORM_LATE)
 
 // Where kernels say that a bounded wait ran out (mam_capi.cu): a flag of the device, and its image in pinned host memory, which
 // kernels that are given its address write too, so that the host sees it without a copy.

@@ -23,6 +23,7 @@ namespace mamb200 {
 template <int PER>
 constexpr int FWD_RING_THREADS = PER == 8 ? 1024 : PER == 16 ? 768 : 640;
 
+
 struct NormFwdParams {
     const void* x;
     const void* residual;      // nullptr: s = x
@@ -219,43 +220,35 @@ struct NormRing {
     int group, groups, stages;
     unsigned slot_bytes;                   // of one tensor's row
     unsigned weights_at, bars_at, bytes;   // the parameters, the barriers; the whole
-    unsigned polls;                        // of a wait for a row, after which it gives up
+    unsigned late;                         // 1: the first wait counts as run out (tests)
 };
 
-// The barrier of a row's group, with a vote: whether any of its threads says so.  All of them get the same answer.
-__device__ __forceinline__ bool group_any(int g, int group, bool mine) {
-    if (group == 32) {
-        __syncwarp();
-        return __any_sync(~0u, mine);
-    }
-    unsigned any;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 p, %3, 0;\n\t"
-        "bar.red.or.pred q, %1, %2, p;\n\t"
-        "selp.u32 %0, 1, 0, q;\n\t}"
-        : "=r"(any)
-        : "r"(g + 1), "r"(group), "r"((unsigned)mine)
-        : "memory");
-    return any != 0;
-}
+constexpr unsigned RING_POLLS = 1u << 22;      // of a wait for a row; each may suspend the thread for a while
 
-// What a group does when a wait for a row ran out, as the vote behind it tells all its threads: the results are void, the flag
-// says so, and the group leaves its loop without arming a barrier or sending for a row again.  The copies that are on
-// their way, of `sent` rows from `row` on, write to this CTA's shared memory and are waited for (at length, one thread)
-// before the CTA may reuse or leave it.
-__device__ __forceinline__ void ring_give_up(uint64_t* full, int stages, int stage, unsigned phase, int sent, long long row,
-                                             long long step, long long rows, const WaitWords& w) {
+// A wait for a row ran out.  The results are void, which the flag says; the thread waits no more, but it meets every barrier of its
+// group.  Where it is thread 0, which arms the barriers and sends for the rows, that ends here too (a barrier whose copy is
+// pending must not be armed again), and it waits for the copies on their way, of `sent` rows from `row` on: they write
+// to shared memory that the CTA may reuse or leave.  Another thread needs no such care: its stage is sent for again only
+// behind its group's barrier, after thread 0 has seen it full.
+__device__ __forceinline__ void ring_late(const WaitWords& w, uint64_t* full, int stages, int stage, unsigned phase, int sent,
+                                          long long row, long long step, long long rows) {
     *w.flag = 1;
     *reinterpret_cast<volatile int*>(w.image) = 1;
     __threadfence_system();
     for (int k = 0; k < sent && row < rows; ++k, row += step) {
-        mbar_wait_bounded(full + stage, phase);
+        mbar_wait_bounded(full + stage, phase, RING_POLLS);
         if (++stage == stages) {
             stage = 0;
             phase ^= 1;
         }
     }
+}
+// The same as a call: in the forward's kernels the code in line cost the loop its schedule ([32768,4096] bf16 behind a residual
+// 205 us, with the call 180); in the backward's it is the faster one ([5003,1283] bf16 38.5 us for 40.3, [16384,5120] 170.6 for
+// 175.5, with dropout and residual).
+__device__ __noinline__ void ring_late_call(const WaitWords& w, uint64_t* full, int stages, int stage, unsigned phase, int sent,
+                                            long long row, long long step, long long rows) {
+    ring_late(w, full, stages, stage, phase, sent, row, step, rows);
 }
 
 // Many rows that are ragged, or too wide for the next kernel's loads to be held: one CTA an SM walks them with the parameters
@@ -330,9 +323,14 @@ mam_norm_fwd_ring_kernel(const __grid_constant__ NormFwdParams p, const __grid_c
     uint4 carry = make_uint4(0u, 0u, 0u, 0u);
     int stage = 0;
     unsigned phase = 0;
+    bool lost = ring.late;
+    if (lost) ring_late_call(p.wait, full, ring.stages, 0, 0, t == 0 ? ring.stages : 0, row, step, p.rows);
     for (; row < p.rows; row += step, at += at_step, start += drop_step) {
         unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
-        const bool late = !mbar_wait_bounded(full + stage, phase, ring.polls);
+        if (!lost && !mbar_wait_bounded(full + stage, phase, RING_POLLS)) {
+            lost = true;
+            ring_late_call(p.wait, full, ring.stages, stage, phase, t == 0 ? ring.stages : 0, row, step, p.rows);
+        }
         unsigned skip_x = 0, skip_r = 0;
         if constexpr (MODE == RAGGED) {
             const T *px = x0 + row * p.x_pitch, *pr = r0 + row * p.res_pitch;
@@ -375,12 +373,9 @@ mam_norm_fwd_ring_kernel(const __grid_constant__ NormFwdParams p, const __grid_c
         }
         float mu = lane_sum<32>(sum2(s));
         if (warps > 1 && lane == 0) slot[0][threadIdx.x >> 5].x = mu;
-        if (group_any(g, group, late)) {
-            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages, row, step, p.rows, p.wait);
-            break;
-        }
+        meet();
         // all have this row in their registers
-        if (t == 0) send(row + ring.stages * step, stage);
+        if (t == 0 && !lost) send(row + ring.stages * step, stage);
         if (warps > 1) mu = lane_sum<MOST>(lane < warps ? slot[0][slot0 + lane].x : 0.f);
         mu *= p.inv_width;
         const float2 minus = splat2(-mu);
@@ -725,13 +720,17 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
     float2 next = row < p.rows ? p.stats[row] : make_float2(0.f, 0.f);
     int stage = 0;
     unsigned phase = 0, parity = 0;
-    bool lost = false;
+    bool lost = ring.late;
+    if (lost) ring_late(p.wait, full, ring.stages, 0, 0, t == 0 ? ring.stages - 1 : 0, row, step, p.rows);
     for (; row < p.rows; row += step, at += at_step, start += drop_step) {
         const float2 st = next;
         if (row + step < p.rows) next = p.stats[row + step];
         const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
         const unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
-        const bool late = !mbar_wait_bounded(full + stage, phase, ring.polls);
+        if (!lost && !mbar_wait_bounded(full + stage, phase, RING_POLLS)) {
+            lost = true;
+            ring_late(p.wait, full, ring.stages, stage, phase, t == 0 ? ring.stages - 1 : 0, row, step, p.rows);
+        }
         float2 h[NV][V / 2], a[NV][V / 2], s1 = splat2(0.f), s2 = s1;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -762,15 +761,15 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
                 }
             }
         float2 m = lane_sum2<32>(sum2(s1), sum2(s2));
-        // two sets of slots in turn: a set is written again only behind the next row's barrier
-        if (warps > 1 && lane == 0) slot[parity][threadIdx.x >> 5] = m;
-        if (group_any(g, group, late)) {
-            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait);
-            lost = true;
-            break;
+        if (warps > 1) {
+            // two sets of slots in turn: a set is written again only behind the next row's barrier
+            if (lane == 0) slot[parity][threadIdx.x >> 5] = m;
+            asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
+        } else {
+            __syncwarp();
         }
         // all have left the row before this one: its stage takes the row stages - 1 ahead
-        if (t == 0) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
+        if (t == 0 && !lost) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
         if (warps > 1) {
             m = (lane & (MOST - 1)) < warps ? slot[parity][slot0 + (lane & (MOST - 1))] : make_float2(0.f, 0.f);
             m = lane_sum2<MOST>(m.x, m.y);
@@ -808,7 +807,7 @@ mam_norm_bwd_ring_kernel(const __grid_constant__ NormBwdParams p, const __grid_c
     }
     if (!p.partial) return;
     float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
-    // the groups' sums meet in the ring's memory, where no copy is on its way any more (unless a wait gave up): a fixed order
+    // the groups' sums meet in the ring's memory, where no copy is on its way any more (unless a wait ran out): a fixed order
     if (__syncthreads_or(lost)) return;
     float* cols = reinterpret_cast<float*>(smem);
     float* to = groups > 1 ? cols + (size_t)g * 2 * width : out;
@@ -909,7 +908,8 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
     uint4 carry = make_uint4(0u, 0u, 0u, 0u), carry2 = carry;
     int stage = 0;
     unsigned phase = 0, parity = 0;
-    bool lost = false;
+    bool lost = ring.late;
+    if (lost) ring_late(p.wait, full, ring.stages, 0, 0, t == 0 ? ring.stages - 1 : 0, row, step, p.rows);
     auto meet = [&]() {
         if (warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(g + 1), "r"(group) : "memory");
         else __syncwarp();
@@ -919,7 +919,10 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
         if (row + step < p.rows) next = p.stats[row + step];
         const float2 minus = splat2(-st.x), r2 = splat2(st.y);    // (s - mu) r in this order: exact where s is near mu
         unsigned char* from = mine + (size_t)stage * TENSORS * ring.slot_bytes;
-        const bool late = !mbar_wait_bounded(full + stage, phase, ring.polls);
+        if (!lost && !mbar_wait_bounded(full + stage, phase, RING_POLLS)) {
+            lost = true;
+            ring_late(p.wait, full, ring.stages, stage, phase, t == 0 ? ring.stages - 1 : 0, row, step, p.rows);
+        }
         const T *ps = s0 + row * p.s_pitch, *py = gy0 + at, *pz = gs0 + at;
         if (edge(row)) {
             T *ds = reinterpret_cast<T*>(from + misfit(ps)), *dy = reinterpret_cast<T*>(from + ring.slot_bytes + misfit(py)),
@@ -971,13 +974,9 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
         float2 m = lane_sum2<32>(sum2(s1), sum2(s2));
         // two sets of slots in turn: a set is written again only behind the next row's barrier
         if (warps > 1 && lane == 0) slot[parity][threadIdx.x >> 5] = m;
-        if (group_any(g, group, late)) {
-            if (t == 0) ring_give_up(full, ring.stages, stage, phase, ring.stages - 1, row, step, p.rows, p.wait);
-            lost = true;
-            break;
-        }
+        meet();
         // all have left the row before this one: its stage takes the row stages - 1 ahead
-        if (t == 0) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
+        if (t == 0 && !lost) send(row + (ring.stages - 1) * step, stage == 0 ? ring.stages - 1 : stage - 1);
         if (warps > 1) {
             m = (lane & (MOST - 1)) < warps ? slot[parity][slot0 + (lane & (MOST - 1))] : make_float2(0.f, 0.f);
             m = lane_sum2<MOST>(m.x, m.y);
@@ -1025,7 +1024,7 @@ mam_norm_bwd_ragged_kernel(const __grid_constant__ NormBwdParams p, const __grid
     }
     if (!p.partial) return;
     float* out = p.partial + (long long)blockIdx.x * 2 * p.width;
-    // the groups' sums meet in the ring's memory, where no copy is on its way any more (unless a wait gave up): a fixed order
+    // the groups' sums meet in the ring's memory, where no copy is on its way any more (unless a wait ran out): a fixed order
     if (__syncthreads_or(lost)) return;
     float* cols = reinterpret_cast<float*>(smem);
     float* to = groups > 1 ? cols + (size_t)g * 2 * width : out;

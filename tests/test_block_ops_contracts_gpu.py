@@ -96,13 +96,13 @@ def test_copies_of_a_module_drop_their_own_elements_in_a_captured_graph(cuda):
 
 
 @pytest.fixture
-def ring_wait():
-    """Sets after how many polls a norm's wait for a row gives up; the library's own limit afterwards."""
+def late():
+    """Whether a norm's first wait for a row counts as run out, for every group of threads and with its copies on their way."""
     from mamtorch_b200 import _lib
 
     L = _lib.lib()
-    yield lambda polls: _lib.check(L.mam_tune_set(6, polls), "mam_tune_set")
-    _lib.check(L.mam_tune_set(6, -1), "mam_tune_set")
+    yield lambda on: _lib.check(L.mam_tune_set(6, int(on)), "mam_tune_set")
+    _lib.check(L.mam_tune_set(6, 0), "mam_tune_set")
     L.mam_check_device_flag()
 
 
@@ -112,13 +112,9 @@ RING_SHAPES = [(3000, 131), (3000, 1283), (2400, 8191), (3000, 136), (3000, 768)
 
 @pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape", RING_SHAPES)
-def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable(cuda, ring_wait, shape, t):
-    """Limits of no poll (every group gives up at its first row, with its copies on their way) and of one (at any row, or at
-    none)."""
-    from mamtorch_b200 import _lib
+def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable(cuda, late, shape, t):
     from mamtorch_b200.nn import functional as MF
 
-    L = _lib.lib()
     rows, width = shape
     x, r, gy = (torch.randn(rows, width, device=cuda).to(t) for _ in range(3))
     x.requires_grad_()
@@ -130,31 +126,28 @@ def test_a_wait_that_runs_out_is_reported_and_leaves_the_device_usable(cuda, rin
     def grads(outs):
         return torch.autograd.grad(outs, (x, w, b), (gy, gy, gy))
 
-    def step():
-        outs = forward()
-        return [*outs, *grads(outs)]
-
-    want = step()
+    want = forward()
+    want += grads(want)
     MF.check_device_flag()
-    for polls in (0, 1, 0, 1):
-        outs = forward()           # the forward's wait is the library's own
-        for call, ref in ((lambda: grads(outs), want[3:]), (step, want)):     # noqa: B023
-            ring_wait(polls)
-            try:
-                got = call()       # a later call in it may find what an earlier one left
+    for _ in range(3):
+        outs = forward()
+        for call in (lambda: grads(outs), lambda: grads(forward())):     # noqa: B023
+            late(True)
+            with pytest.raises(RuntimeError, match="gave up"):
+                call()       # a later call in it may find what an earlier one left
                 MF.check_device_flag()
-                assert polls > 0
-                assert all(torch.equal(p, q) for p, q in zip(got, ref))
-            except RuntimeError as e:
-                assert "gave up" in str(e)
+            late(False)
             torch.cuda.synchronize()
-            L.mam_check_device_flag()
-        ring_wait(-1)
-        assert all(torch.equal(p, q) for p, q in zip(step(), want))
+            try:
+                MF.check_device_flag()
+            except RuntimeError as e:      # a kernel that was launched before the report
+                assert "gave up" in str(e)
+        outs = forward()
+        assert all(torch.equal(p, q) for p, q in zip([*outs, *grads(outs)], want))
         MF.check_device_flag()
 
 
-def test_a_forward_whose_wait_runs_out_is_reported(cuda, ring_wait):
+def test_a_forward_whose_wait_runs_out_is_reported(cuda, late):
     from mamtorch_b200.nn import functional as MF
 
     # ragged rows, and wide 16-bit ones behind a residual: the forward's forms through shared memory
@@ -162,16 +155,16 @@ def test_a_forward_whose_wait_runs_out_is_reported(cuda, ring_wait):
         x, r = (torch.randn(shape, device=cuda).to(t) for _ in range(2))
         call = (lambda: MF.dropout_add_layer_norm(x, r, drop_rate=0.1, drop_seed=5)) if add else (lambda: (MF.layer_norm(x),))   # noqa: B023
         want = call()
-        ring_wait(0)
+        late(True)
         call()
         with pytest.raises(RuntimeError, match="gave up"):
             MF.check_device_flag()
-        ring_wait(-1)
+        late(False)
         assert all(torch.equal(p, q) for p, q in zip(call(), want))
         MF.check_device_flag()
 
 
-def test_the_next_call_of_the_norm_reports_a_wait_that_ran_out(cuda, ring_wait):
+def test_the_next_call_of_the_norm_reports_a_wait_that_ran_out(cuda, late):
     from mamtorch_b200.nn import functional as MF
 
     x = torch.randn(3000, 1283, device=cuda, requires_grad=True)     # ragged rows: the forward and the backward wait
@@ -180,10 +173,10 @@ def test_the_next_call_of_the_norm_reports_a_wait_that_ran_out(cuda, ring_wait):
     want = MF.layer_norm(few)
 
     def left_behind(call):
-        ring_wait(0)
+        late(True)
         call()
         torch.cuda.synchronize()
-        ring_wait(-1)
+        late(False)
 
     y = MF.layer_norm(x)
     for call in (lambda: MF.layer_norm(x.detach()), lambda: torch.autograd.grad(y, x, gy, retain_graph=True),
@@ -205,7 +198,7 @@ def test_the_next_call_of_the_norm_reports_a_wait_that_ran_out(cuda, ring_wait):
         MF.layer_norm(few)
     graph.replay()
     torch.cuda.synchronize()
-    MF.check_device_flag()      # captured with the library's own limit
+    MF.check_device_flag()      # captured without the hook
     assert torch.equal(z, y)
 
 
