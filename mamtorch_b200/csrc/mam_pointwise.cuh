@@ -22,17 +22,18 @@ struct PointParams {
 enum PointOp { POINT_DROPOUT, POINT_GELU, POINT_GELU_BWD };
 
 // q = -erfc(a / sqrt(2)) / 2 and e = exp(-a^2 / 2) for a = min(|x|, 15), pairwise: the form of Abramowitz and Stegun, 7.1.26,
-// t P(t) e with t = 1 / (1 + 0.28 a), P with six coefficients of our own fit instead of five (largest error of the
-// coefficients as they stand 1.1e-8, at a = 1.09; roundings make it 2e-7 at a = 0, where the sum to 0.5 counts).  erff and
-// expf took 33 instructions an element and twice the time of the bytes in bf16; this takes a reciprocal, an exponential and
-// the rest in packed pairs.  15: beyond it q is zero in fp32; min.NaN passes a NaN on.
+// t P(t) e with t = 1 / (1 + k a), and coefficients of our own fits.  erff and expf took 33 instructions an element and twice
+// the time of the bytes in bf16; this takes a reciprocal, an exponential and the rest in packed pairs.  15: beyond it q is
+// zero in fp32; min.NaN passes a NaN on.
 //
-// fp32 takes another form of q where a < 1: there q is of the order of one half, and its absolute error shows (x Phi(x) off by
-// 4.7e-7 relative, erff's form by 2.1e-7; with this 2.7e-7; from 1 on 8e-8 absolute on the negative side, erff's form
-// 1.2e-7).  q = a P(a^2) - 1/2, P a polynomial of our own fit, off by 3.1e-8 relative to q with its rounded coefficients.  The form
-// that counts is taken by products, not by selects, whose pipe is the busier one: the weight 2^25 (1 - a), saturated,
-// is exactly 1 below a = 1 and 0 from there on, and the difference of two such close numbers is exact.  12608x4096, with
-// dropout: forward 61.9 -> 65.1 us, backward 90.5 -> 89.2, and 61.6 without (erff and expf: 87 and 115, 68 without).
+// 16-bit types: k = 0.28, six coefficients (as they stand off by 1.1e-8 at most, at a = 1.09; roundings make it 2e-7 at
+// a = 0, where q is of the order of one half).
+// fp32: there that absolute error would show (x Phi(x) off by 4.7e-7 relative, rms 1.0e-7, where erff's form has 2.2e-7 and 4.6e-8),
+// and for a < 1 q = a R(a^2) - 1/2, R a polynomial, off by 7e-9.  From a = 1 on R's form is too high, more and more so; the
+// other one, k = 0.37 with five coefficients fitted from a = 1 on (a q off by 4.6e-9), is too high below it, by more than
+// its roundings from 0.9 down.  So the lower of the two is the one that counts, and close to 1 either is: 2.9e-7, rms 4.0e-8.
+// 12608x4096 with dropout, forward and backward: 151.5 -> 150.2 us; under load for seconds, where the power limit takes the
+// clock to 1.5 GHz and instructions count, 163.7 -> 173.5 (28.2 -> 31.5 and 31.3 -> 35.2 an element).  erff and expf took 202.
 template <typename T>
 __device__ __forceinline__ void normal_tail(float2 x, float2& a, float2& q, float2& e) {
     float u, v;
@@ -40,30 +41,33 @@ __device__ __forceinline__ void normal_tail(float2 x, float2& a, float2& q, floa
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(u) : "f"(fabsf(u)), "f"(15.f));
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(fabsf(v)), "f"(15.f));
     a = make_float2(u, v);
-    split2(fma2(a, splat2(0.28f), splat2(1.f)), u, v);
+    split2(fma2(a, splat2(sizeof(T) == 2 ? 0.28f : 0.37f), splat2(1.f)), u, v);
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(u));
     asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v));
-    const float2 t = make_float2(u, v);
-    split2(mul2(mul2(a, a), splat2(-0.72134752044448170f)), u, v);    // -a^2 / 2 in base 2
+    const float2 t = make_float2(u, v), aa = mul2(a, a);
+    split2(mul2(aa, splat2(-0.72134752044448170f)), u, v);    // -a^2 / 2 in base 2
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(u));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(v));
     e = make_float2(u, v);
-    float2 s = fma2(splat2(0.105807796f), t, splat2(-0.389872253f));
-    s = fma2(s, t, splat2(0.23699066f));
-    s = fma2(s, t, splat2(-0.268907934f));
-    s = fma2(s, t, splat2(-0.0674976185f));
-    s = fma2(s, t, splat2(-0.116520643f));
-    q = mul2(mul2(s, t), e);
-    if constexpr (sizeof(T) == 4) {
-        s = mul2(a, a);
-        float2 p = fma2(splat2(9.171009151032194e-05f), s, splat2(-0.0011636228300631046f));
-        p = fma2(p, s, splat2(0.009962853975594044f));
-        p = fma2(p, s, splat2(-0.0664883628487587f));
-        p = fma2(p, s, splat2(0.39894217252731323f));
-        split2(a, u, v);
-        u = __saturatef(fmaf(u, -33554432.f, 33554432.f));
-        v = __saturatef(fmaf(v, -33554432.f, 33554432.f));
-        q = fma2(make_float2(u, v), fma2(q, splat2(-1.f), fma2(a, p, splat2(-0.5f))), q);
+    if constexpr (sizeof(T) == 2) {
+        float2 s = fma2(splat2(0.105807796f), t, splat2(-0.389872253f));
+        s = fma2(s, t, splat2(0.23699066f));
+        s = fma2(s, t, splat2(-0.268907934f));
+        s = fma2(s, t, splat2(-0.0674976185f));
+        s = fma2(s, t, splat2(-0.116520643f));
+        q = mul2(mul2(s, t), e);
+    } else {
+        float2 s = fma2(splat2(0.10187085717916489f), t, splat2(-0.23629137873649597f));
+        s = fma2(s, t, splat2(-0.05451401323080063f));
+        s = fma2(s, t, splat2(-0.16487039625644684f));
+        s = fma2(s, t, splat2(-0.14599835872650146f));
+        s = mul2(mul2(s, t), e);
+        float2 r = fma2(splat2(9.171009151032194e-05f), aa, splat2(-0.0011636228300631046f));
+        r = fma2(r, aa, splat2(0.009962853975594044f));
+        r = fma2(r, aa, splat2(-0.0664883628487587f));
+        r = fma2(r, aa, splat2(0.39894217252731323f));
+        r = fma2(a, r, splat2(-0.5f));
+        q = make_float2(fminf(r.x, s.x), fminf(r.y, s.y));      // a NaN is in both
     }
 }
 // x Phi(x) = max(x, 0) + |x| q: zero at minus infinity, its limit
@@ -78,24 +82,15 @@ __device__ __forceinline__ float2 gelu2(float2 x) {
 __device__ __forceinline__ float flip(float u, float sign) {
     return __uint_as_float(__float_as_uint(u) ^ (__float_as_uint(sign) & 0x80000000u));
 }
-// Phi(x) + x phi(x).  16-bit types: 1/2 + sign(x) (1/2 + q + a phi(a)).  fp32: q + a phi(a) with the sign of x, and one more for
-// a positive x, so that the negative side keeps its digits.
+// Phi(x) + x phi(x) = 1/2 + sign(x) (1/2 + q + a phi(a))
 template <typename T>
 __device__ __forceinline__ float2 gelu_slope2(float2 x) {
     float2 a, q, e;
     normal_tail<T>(x, a, q, e);
-    const float2 c = splat2(0.39894228040143268f);
     float u, v, xu, xv;
+    split2(add2(fma2(mul2(a, splat2(0.39894228040143268f)), e, splat2(0.5f)), q), u, v);
     split2(x, xu, xv);
-    if constexpr (sizeof(T) == 2) {
-        split2(add2(fma2(mul2(a, c), e, splat2(0.5f)), q), u, v);
-        return add2(make_float2(flip(u, xu), flip(v, xv)), splat2(0.5f));
-    } else {
-        split2(fma2(mul2(a, c), e, q), u, v);
-        // by the sign bit: minus zero goes with the negative side
-        return add2(make_float2(flip(u, xu), flip(v, xv)),
-                    make_float2(__float_as_int(xu) < 0 ? 0.f : 1.f, __float_as_int(xv) < 0 ? 0.f : 1.f));
-    }
+    return add2(make_float2(flip(u, xu), flip(v, xv)), splat2(0.5f));
 }
 
 template <typename T, int OP, int N>

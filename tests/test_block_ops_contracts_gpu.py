@@ -235,15 +235,14 @@ def test_the_first_call_of_a_process_inside_a_capture(cuda):
 def test_gelu_over_a_dense_grid(cuda, n, t):
     """The elementwise error of GELU and its slope on [-15, 15], in eps = 2^-24, half a step of fp32.
 
-    fp32, |x| < 1: Phi(-a) = 1/2 - a P, a = |x|.  P's roundings are 1.36 eps of P (its last step one, the step before and a^2 damped
-    by the coefficients), a P / Phi(-a) is 2.15 at most, the coefficients are off by 1.4 eps relative to Phi(-a), it rounds once,
-    and so does its product with a: 2.15 * 1.36 + 1.4 + 2 = 6.4 eps relative.  The slope's a P - 1/2 + a c e: 1.36 eps a P + eps / 4,
-    a c e within 1.5 eps (e = ex2, two units in the last place, its argument twice rounded, times 0.242; a c), the sum eps / 4, and
-    one more added, eps: 3.5 eps.
+    fp32, a = |x| < 0.85: q = -Phi(-a) = a R - 1/2.  R's roundings are 1.36 eps of R (its last step one, the step before and a^2
+    damped by the coefficients), a R / Phi(-a) is 2.15 at most (at 1), the coefficients are off by 0.1 eps, q rounds once, and so
+    does its product with a: 2.15 * 1.36 + 0.6 + 2 = 5.6 eps relative.  The slope's sum a c e + 1/2 + q: a c e within 1.5 eps (e = ex2,
+    two units in the last place, its argument twice rounded; a c), two additions, q within 1.36 eps a R + eps / 4: 3.6 eps.
     Elsewhere, and in 16-bit types everywhere, Phi(-a) = s(t) t e: t within 3 eps (sum, reciprocal), each step of s one eps of its
-    value, e as above, two products, the fit 1.1e-8: a Phi(-a) within 3.2 eps for a >= 1 and 3.4 for all a, the slope's sum
-    within 4.8 eps for a >= 1, and 12 for all a, where 1/2 is added twice to sums of the order of one.  Then one rounding to
-    fp32 relative to the value, one to t, and the product with the upstream gradient, which is one."""
+    value, e as above, two products, and the coefficients: a Phi(-a) within 3.2 eps, 3.4 in 16-bit types, the slope's sum within
+    5.8 eps, 12 in 16-bit types.  Then one rounding to fp32 relative to the value, one to t, and the product with the upstream
+    gradient, which is one."""
     from mamtorch_b200.nn import functional as MF
 
     eps, half = 2.0 ** -24, torch.finfo(t).eps / 2
@@ -254,16 +253,16 @@ def test_gelu_over_a_dense_grid(cuda, n, t):
     phi = 0.5 * torch.erfc(-z / math.sqrt(2))
     want, slope = z * phi, phi + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     tiny = torch.finfo(t).smallest_normal * torch.finfo(t).eps
-    near = (z.abs() < 1) & (t == torch.float32)
-    far_y, far_slope = (3.2, 4.8) if t == torch.float32 else (3.4, 12.0)
+    near = (z.abs() < 0.85) & (t == torch.float32)
+    far_y, far_slope = (3.2, 5.8) if t == torch.float32 else (3.4, 12.0)
     rounded = 0.0 if t == torch.float32 else half
-    bound = torch.where(near, 6.4 * eps * want.abs(), far_y * eps + eps * want.abs()) + rounded * want.abs() + tiny
+    bound = torch.where(near, 5.6 * eps * want.abs(), far_y * eps + eps * want.abs()) + rounded * want.abs() + tiny
     assert ((y.detach().double() - want).abs() - bound).max().item() <= 0
-    bound = torch.where(near, 3.5 * eps, far_slope * eps + eps * slope.abs()) + rounded * slope.abs() + tiny
+    bound = torch.where(near, 3.6 * eps, torch.full_like(slope, far_slope * eps)) + (eps + rounded) * slope.abs() + tiny
     assert ((dx.double() - slope).abs() - bound).max().item() <= 0
     if t == torch.float32:      # no less exact than the erff form that it stands for: 10 % for the grid's luck
         other = torch.nn.functional.gelu(x.detach()).double()
-        middle = near & (z != 0)
+        middle = (z.abs() < 1) & (z != 0)
         rms = lambda v: ((v - want)[middle] / want[middle]).square().mean().sqrt().item()   # noqa: E731
         assert rms(y.detach().double()) <= 1.1 * rms(other)
         assert (y.detach().double() - want).abs().max() <= (other - want).abs().max()
