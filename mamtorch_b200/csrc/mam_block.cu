@@ -143,7 +143,8 @@ int fwd_pick(NormFwdParams& p, bool aligned, const DevInfo& d, cudaStream_t st) 
     const bool few = p.rows < 4 * (long long)d.sms;
     // Through shared memory: ragged rows (bf16 [5003, 1283] 18.5 -> 16.5 us, with dropout and residual 45 -> 30), and 16-bit rows
     // behind a residual that would take eight vectors a thread ([32768, 4096] 277 -> 179 us).  The others keep more
-    // threads on an SM without it: [32768, 4096] bf16 97 us against 118, [12608, 768] fp32 with residual 27 against 29.
+    // threads on an SM without it: [32768, 4096] bf16 97 us against 118, [12608, 768] fp32 with residual 27 against 29; 16-bit
+    // with residual, without / through shared memory: [16384, 5120] 124 / 132, [32768, 2560] 114 / 123, 1280 63 / 74, 1024 47 / 51.
     const bool eight = vecs > 192 && (vecs <= 256 || vecs % 256 == 0 || vecs > 2048);
     if ((!aligned || (ADD && eight && sizeof(T) == 2)) && p.rows >= 16LL * d.sms && p.width > 128) {
         const FwdPlan b = fwd_plan(p.width, sizeof(T), ADD, aligned, d);

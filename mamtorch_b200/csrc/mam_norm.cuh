@@ -1202,8 +1202,9 @@ mam_norm_bwd_cols_kernel(const __grid_constant__ NormBwdParams p, long long rows
 }
 
 // dw and db: the partial rows added in a fixed order, rounded once to the parameters' type.  Bound by the latency of its
-// loads: eight rows at a time in a CTA, eight of them in flight a thread.  It is launched while the kernel before it still
-// runs, and waits for that one's partial rows here.
+// loads: eight rows at a time in a CTA, eight of them in flight a thread.  Its launch depends programmatically on the kernel
+// before it, which has no early trigger: it starts when that kernel's last CTA has ended and waits here for its partial
+// rows.  What that saves is a part of the gap between two launches: [12608, 768] fp32 25.5 us for 26.2, [8192, 2048] bf16 nothing.
 template <typename T>
 __global__ void __launch_bounds__(NORM_COLS * NORM_LANES)
 mam_norm_params_kernel(const float* partial, void* dweight, void* dbias, long long parts, long long width,
