@@ -113,7 +113,8 @@ class MAMMlpBlock(nn.Module):
     ViT-B/16: hidden 768, intermediate 3072, 197 tokens per image.
 
     `fused=True` runs norm, GELU and residual in this library's kernels (equal to torch's up to rounding) and allows
-    `drop_rate`: dropout behind the GELU and before the residual, in training, with masks that are never stored."""
+    `drop_rate`: dropout behind the GELU and before the residual, in training, with masks that are never stored.  `norm` then
+    lends its weight, bias and eps; it and `act` are not called as modules (their hooks do not run)."""
 
     def __init__(self, hidden: int = 768, intermediate: int = 3072, vcon_steps: int = 0, vcon_type: str = "linear",
                  store_args: bool = False, residual: bool = True, layer_norm_eps: float = 1e-12, device=None,
@@ -161,7 +162,8 @@ class MAMMlpBlock(nn.Module):
 
 class MAMMlpStack(nn.Module):
     """`depth` fused MLP blocks and the final norm of the encoder (`vit.layernorm` of a Hugging Face ViT):
-    LayerNorm(block_depth(... block_1(x))).  The residual stream and the next norm's output come out of one pass."""
+    LayerNorm(block_depth(... block_1(x))).  The residual stream and the next norm's output come out of one pass, so the
+    blocks and norms are not called as modules themselves (the MAM layers in them are)."""
 
     def __init__(self, depth: int, hidden: int = 768, intermediate: int = 3072, layer_norm_eps: float = 1e-12,
                  drop_rate: float = 0.0, device=None, dtype=None, **block_kwargs):
